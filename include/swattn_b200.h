@@ -321,6 +321,59 @@ int swa_prefill_forward_noalloc(const void* q, const void* k, const void* v, con
                                 void* out, float* lse, int B, int Sq, int Skv, int Hq, int Hkv, int head_dim,
                                 int window, float scale_log2, int32_t* status_out, void* stream);
 
+/* Block-scaled 8-bit KV cache (no counterpart in the reference, which is prefill
+ * only).  k_cache / v_cache: [B, Hkv, Smax, 128] bytes (dtype: SWA_KV_E4M3 or
+ * SWA_KV_INT8), the rows of a KV head together; k_scale / v_scale: fp32 [B, Hkv, nblk],
+ * nblk = ceil(Smax / block_size), one non-negative scale per block of block_size (16,
+ * 32, 64 or 128) rows of a head: value = byte * scale.  seq_lens: device int32 [B], the
+ * cached rows of each sequence (clamped to [0, Smax]); key_weights: fp32 [B, Hkv, Smax].
+ * Rows from a sequence's length on are neither read for their values nor written,
+ * except the new ones.  Calls on one cache are ordered by the caller (one stream). */
+#define SWA_KV_E4M3 1
+#define SWA_KV_INT8 2
+
+/* Appends rows.  k_new / v_new: bf16, element (b, t, g, d) at b * strides[0] + t *
+ * strides[1] + g * strides[2] + d (host arrays of 3 element strides, multiples of 8),
+ * 0 <= t < T.  Rows t < n_b (new_lens[b] clamped to [0, T]; new_lens NULL: T) of sequence
+ * b become cache rows start[b] + t (those at Smax and past it are dropped), and
+ * seq_lens[b] the end of them; start may be seq_lens.  Each touched block's scale
+ * becomes the smallest power of two (at least 2^-126; 0 for a block of zeros) that both
+ * its earlier rows' scale and the largest finite |value| of its new rows need (448 /
+ * 127 times it reaches them); earlier rows of the block are rounded again when it
+ * differs from what it was.  Values are rounded to nearest even; infinities saturate,
+ * NaN stays NaN (e4m3) or becomes 0 (int8).  key_weights (nullable): new rows start at 0. */
+int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides, const int64_t* v_strides,
+                  const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
+                  float* v_scale, float* key_weights, int32_t* seq_lens, int B, int T, int Hkv, int Smax,
+                  int head_dim, int block_size, int dtype, void* stream);
+
+/* Decode step over the cache: as swa_decode_forward, with q's element (b, h, d) at b *
+ * q_stride_b + h * q_stride_h + d (multiples of 8).  key_weights (nullable): the
+ * attention weight of each legal key, summed over the query heads of its group, is
+ * added to it.  The workspace's first int32 is the status word (0 or
+ * SWA_STATUS_TIMEOUT), valid once the call has run; the workspace needs no clearing
+ * and calls that may overlap need one each. */
+size_t swa_kv_decode_workspace_bytes(int B, int Smax, int Hq, int Hkv, int with_weights);
+int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache, const void* v_cache,
+                  const float* k_scale, const float* v_scale, const int32_t* seq_lens, const uint8_t* route,
+                  void* out, float* lse, float* key_weights, int B, int Smax, int Hq, int Hkv, int head_dim,
+                  int block_size, int window, float scale_log2, int dtype, void* workspace, size_t workspace_bytes,
+                  void* stream);
+
+/* Evicts rows.  A sequence with at most `keep` rows keeps them all.  Of a longer one
+ * every KV head keeps its first `sink` and last `recent` rows and, of those between,
+ * the keep - sink - recent with the largest key_weights (ties: the lowest row first;
+ * NaN: last), moved together in their order.  The destination is the source itself (all
+ * six pointers equal) or shares nothing with it and has Smax_out >= min(keep, Smax)
+ * rows.  A destination block's scale is the largest of its rows' scales; rows of
+ * another scale are rounded again.  slots: int32 [B, Hkv, min(keep, Smax)], the source
+ * row of each kept row, -1 past the kept ones. */
+int swa_kv_evict(const void* k_cache, const void* v_cache, const float* k_scale, const float* v_scale,
+                 const float* key_weights, const int32_t* seq_lens, void* k_out, void* v_out, float* k_scale_out,
+                 float* v_scale_out, float* key_weights_out, int32_t* seq_lens_out, int32_t* slots, int B, int Hkv,
+                 int Smax, int Smax_out, int head_dim, int block_size, int keep, int sink, int recent, int dtype,
+                 void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -24,6 +24,8 @@ STATUS_COVER = 1 << 6
 STATUS_TIMEOUT = 1 << 16
 ROUTER_BF16 = 1
 ROUTER_F32 = 2
+KV_E4M3 = 1
+KV_INT8 = 2
 
 EXPORTED = (
     "swa_abi_version",
@@ -52,6 +54,10 @@ EXPORTED = (
     "swa_decode_forward_fp8",
     "swa_prefill_split_plan",
     "swa_prefill_forward_split",
+    "swa_kv_append",
+    "swa_kv_decode_workspace_bytes",
+    "swa_kv_decode",
+    "swa_kv_evict",
 )
 
 _lock = threading.Lock()
@@ -168,6 +174,35 @@ def _declare(lib) -> None:
         fn = getattr(lib, name)
         fn.restype = _i
         fn.argtypes = [_p, _p, _i, _i, _i, _i, _i, _p, _p]  # src, unit_of_slot, n_slots, S, hkv, chunk, row, dst, stream
+    _i64 = ctypes.c_int64
+    lib.swa_kv_append.restype = _i
+    lib.swa_kv_append.argtypes = [
+        _p, _p, ctypes.POINTER(_i64), ctypes.POINTER(_i64),  # k_new, v_new, k_strides[3], v_strides[3]
+        _p, _p,                # start, new_lens
+        _p, _p, _p, _p, _p, _p,  # k_cache, v_cache, k_scale, v_scale, key_weights, seq_lens
+        _i, _i, _i, _i, _i, _i, _i,  # B, T, Hkv, Smax, head_dim, block_size, dtype
+        _p,                    # stream
+    ]
+    lib.swa_kv_decode_workspace_bytes.restype = _sz
+    lib.swa_kv_decode_workspace_bytes.argtypes = [_i, _i, _i, _i, _i]
+    lib.swa_kv_decode.restype = _i
+    lib.swa_kv_decode.argtypes = [
+        _p, _i64, _i64,        # q, q_stride_b, q_stride_h
+        _p, _p, _p, _p, _p, _p,  # k_cache, v_cache, k_scale, v_scale, seq_lens, route
+        _p, _p, _p,            # out, lse, key_weights
+        _i, _i, _i, _i, _i, _i,  # B, Smax, Hq, Hkv, head_dim, block_size
+        _i, _f, _i,            # window, scale_log2, dtype
+        _p, _sz, _p,           # workspace, workspace_bytes, stream
+    ]
+    lib.swa_kv_evict.restype = _i
+    lib.swa_kv_evict.argtypes = [
+        _p, _p, _p, _p, _p, _p,  # k_cache, v_cache, k_scale, v_scale, key_weights, seq_lens
+        _p, _p, _p, _p, _p, _p,  # the destination's
+        _p,                    # slots
+        _i, _i, _i, _i, _i, _i,  # B, Hkv, Smax, Smax_out, head_dim, block_size
+        _i, _i, _i, _i,        # keep, sink, recent, dtype
+        _p,                    # stream
+    ]
     lib.swa_broadcast_bytes.restype = _i
     lib.swa_broadcast_bytes.argtypes = [_p, _sz, _p, _i, _p]  # src, bytes, dsts[], n_dst, stream
 

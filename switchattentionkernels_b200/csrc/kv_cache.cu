@@ -1,0 +1,561 @@
+// Block-scaled 8-bit KV cache: writing new rows (append) and keeping the heaviest
+// rows (evict).  The attention over the cache is in kv_decode_sm100.cu.
+#include <cooperative_groups.h>
+#include <cuda_fp16.h>
+
+#include "kv_cache.h"
+#include "mma_sync.cuh"
+#include "sm100.cuh"
+
+namespace swa {
+
+namespace {
+
+namespace cg = cooperative_groups;
+
+// ---------------------------------------------------------------------------
+// 8-bit formats
+// ---------------------------------------------------------------------------
+// Smallest power of two s (2^-126 .. 2^127) with s * qmax >= a, for qmax = (1 +
+// mant_q / 2^23) 2^exp_q; 0 when a = 0.  Powers of two because then x / s, and the
+// rescaling of a row when its block's scale grows, are exact before the one
+// rounding to 8 bits: e4m3 loses nothing by it, int8 less than one bit, and rows
+// rounded again at every growth (at most once per doubling) do not drift.
+__device__ __forceinline__ float pow2_at_least(float a, int exp_q, uint32_t mant_q) {
+  const uint32_t bits = __float_as_uint(a);
+  if (bits == 0u) return 0.0f;
+  const int e = static_cast<int>(bits >> 23) - 127 - exp_q + ((bits & 0x7FFFFFu) > mant_q ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23);
+}
+
+template <bool kInt8>
+__device__ __forceinline__ float scale_for(float amax) {
+  return kInt8 ? pow2_at_least(amax, 6, 0x7E0000u) : pow2_at_least(amax, 8, 0x600000u);  // 127, 448
+}
+
+// Four values to 8 bits (byte i = value i): to nearest even, saturating at 127 / 448;
+// NaN becomes 0 (int8) or stays NaN (e4m3).
+template <bool kInt8>
+__device__ __forceinline__ uint32_t pack8(float a, float b, float c, float d) {
+  if constexpr (kInt8) {
+    auto q = [](float x) { return static_cast<uint32_t>(min(max(__float2int_rn(x), -127), 127)) & 0xFFu; };
+    return q(a) | (q(b) << 8) | (q(c) << 16) | (q(d) << 24);
+  } else {
+    uint32_t r;
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 l, %2, %1;\n\t"
+        "cvt.rn.satfinite.e4m3x2.f32 h, %4, %3;\n\t"
+        "mov.b32 %0, {l, h};\n\t}"
+        : "=r"(r)
+        : "f"(a), "f"(b), "f"(c), "f"(d));
+    return r;
+  }
+}
+
+// Four cached bytes times `ratio`, rounded back to 8 bits.
+template <bool kInt8>
+__device__ __forceinline__ uint32_t rescale8(uint32_t v, float ratio) {
+  if constexpr (kInt8) {
+    auto x = [v, ratio](int i) { return static_cast<float>(static_cast<int8_t>(v >> (8 * i))) * ratio; };
+    return pack8<true>(x(0), x(1), x(2), x(3));
+  } else {
+    uint32_t lo, hi;
+    e4m3x4_to_f16x2x2(v, lo, hi);
+    const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+    const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+    return pack8<false>(l.x * ratio, l.y * ratio, h.x * ratio, h.y * ratio);
+  }
+}
+
+template <bool kInt8>
+__device__ __forceinline__ uint4 rescale8(uint4 v, float ratio) {
+  return make_uint4(rescale8<kInt8>(v.x, ratio), rescale8<kInt8>(v.y, ratio), rescale8<kInt8>(v.z, ratio),
+                    rescale8<kInt8>(v.w, ratio));
+}
+
+// Largest |x| over the finite values of packed BF16 pairs, as the BF16's bits (the
+// bits of non-negative BF16 values order as the values do).
+__device__ __forceinline__ uint32_t finite_abs_max(uint32_t pair) {
+  uint32_t lo = pair & 0x7FFFu, hi = (pair >> 16) & 0x7FFFu;
+  lo = lo < 0x7F80u ? lo : 0u;
+  hi = hi < 0x7F80u ? hi : 0u;
+  return max(lo, hi);
+}
+__device__ __forceinline__ uint32_t abs_max_bits(uint4 v) {
+  return max(max(finite_abs_max(v.x), finite_abs_max(v.y)), max(finite_abs_max(v.z), finite_abs_max(v.w)));
+}
+
+__device__ __forceinline__ float bf_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
+__device__ __forceinline__ float bf_hi(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
+
+struct RowRange {
+  int start, end;
+};
+__device__ __forceinline__ RowRange append_range(const KvAppendParams& p, int b) {
+  const int s = min(max(p.start[b], 0), p.Smax);
+  const int n = p.new_lens != nullptr ? min(max(p.new_lens[b], 0), p.T) : p.T;
+  return RowRange{s, min(n, p.Smax - s) + s};
+}
+
+// New scale of a block whose new rows reach `amax_bits`: the scale that its earlier
+// rows need (none: 0), raised to what the new rows need.
+template <bool kInt8>
+__device__ __forceinline__ float grown_scale(uint32_t amax_bits, bool has_old, float old_scale) {
+  const float need = scale_for<kInt8>(__uint_as_float(amax_bits << 16));
+  return has_old ? fmaxf(pow2_at_least(old_scale, 0, 0u), need) : need;
+}
+
+// ---------------------------------------------------------------------------
+// append
+// ---------------------------------------------------------------------------
+// Chunks of many rows: one CTA per (block of rows, KV head, K or V, sequence).  Each
+// thread keeps its part of the block's new rows in registers (kPasses x 16 bytes),
+// so the rows are read once: maximum, scale, rounding, store.  HBM-bound: 2 bytes
+// read and 1 written per value.
+constexpr int kAppendThreads = 256;
+
+template <bool kInt8, int kPasses>
+__global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
+  constexpr int kBlock = 16 * kPasses;
+  const int b = blockIdx.z, g = blockIdx.y >> 1, kv = blockIdx.y & 1;
+  const RowRange rg = append_range(p, b);
+  const int blk = rg.start / kBlock + blockIdx.x;
+  const int row0 = blk * kBlock;
+  if (rg.end <= rg.start || row0 >= rg.end) return;
+  const int tid = threadIdx.x;
+  const int c = tid & 15;  // 8 values of a row
+  const int64_t unit = static_cast<int64_t>(b) * p.Hkv + g;
+  const __nv_bfloat16* x = p.x[kv] + b * p.sb[kv] + g * p.sh[kv] + 8 * c;
+  uint8_t* cache = p.cache[kv] + unit * p.Smax * 128;
+  uint4 v[kPasses];
+  uint32_t amax = 0;
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int pos = row0 + 16 * i + (tid >> 4);
+    v[i] = make_uint4(0, 0, 0, 0);
+    if (pos >= rg.start && pos < rg.end)
+      v[i] = *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(pos - rg.start) * p.st[kv]);
+  }
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) amax = max(amax, abs_max_bits(v[i]));
+  __shared__ uint32_t warp_max[kAppendThreads / 32];
+  __shared__ float old_scale_sh;
+  float* scale = p.scale[kv] + unit * p.nblk + blk;
+  amax = __reduce_max_sync(0xffffffffu, amax);
+  if ((tid & 31) == 0) warp_max[tid >> 5] = amax;
+  if (tid == 0) old_scale_sh = *scale;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < kAppendThreads / 32; ++w) amax = max(amax, warp_max[w]);
+  const bool has_old = rg.start > row0;
+  const float old_scale = old_scale_sh;
+  const float s = grown_scale<kInt8>(amax, has_old, old_scale);
+  const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // a power of two: exact
+  if (has_old && s != old_scale) {
+    const float ratio = old_scale / s;
+    for (int i = tid; i < (rg.start - row0) * 8; i += kAppendThreads) {
+      uint4* q = reinterpret_cast<uint4*>(cache + static_cast<int64_t>(row0) * 128) + i;
+      *q = rescale8<kInt8>(*q, ratio);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < kPasses; ++i) {
+    const int pos = row0 + 16 * i + (tid >> 4);
+    if (pos < rg.start || pos >= rg.end) continue;
+    uint2 o;
+    o.x = pack8<kInt8>(bf_lo(v[i].x) * inv, bf_hi(v[i].x) * inv, bf_lo(v[i].y) * inv, bf_hi(v[i].y) * inv);
+    o.y = pack8<kInt8>(bf_lo(v[i].z) * inv, bf_hi(v[i].z) * inv, bf_lo(v[i].w) * inv, bf_hi(v[i].w) * inv);
+    *reinterpret_cast<uint2*>(cache + static_cast<int64_t>(pos) * 128 + 8 * c) = o;
+  }
+  if (tid == 0) *scale = s;
+  if (kv == 0 && p.weights != nullptr && tid < kBlock) {
+    const int pos = row0 + tid;
+    if (pos >= rg.start && pos < rg.end) p.weights[unit * p.Smax + pos] = 0.0f;
+  }
+}
+
+__global__ void kv_advance_kernel(const __grid_constant__ KvAppendParams p) {
+  const int b = blockIdx.x * blockDim.x + threadIdx.x;
+  if (b < p.B) p.seq_lens[b] = append_range(p, b).end;
+}
+
+// One new row per sequence: a CTA per sequence, a warp per (KV head, K or V), 4
+// values per lane.  Latency-bound (a few KB in all); the CTA is the only one that
+// reads its sequence's length, so it also writes the new one and the call is one
+// launch.
+template <bool kInt8>
+__global__ void __launch_bounds__(1024) kv_append_token_kernel(const __grid_constant__ KvAppendParams p) {
+  const int b = blockIdx.x, lane = threadIdx.x & 31;
+  const RowRange rg = append_range(p, b);
+  if (rg.end > rg.start) {
+    const int blk = rg.start / p.block, row0 = blk * p.block;
+    for (int u = threadIdx.x >> 5; u < 2 * p.Hkv; u += blockDim.x >> 5) {
+      const int g = u >> 1, kv = u & 1;
+      const int64_t unit = static_cast<int64_t>(b) * p.Hkv + g;
+      uint8_t* cache = p.cache[kv] + unit * p.Smax * 128;
+      float* scale = p.scale[kv] + unit * p.nblk + blk;
+      const uint2 v = *reinterpret_cast<const uint2*>(p.x[kv] + b * p.sb[kv] + g * p.sh[kv] + 4 * lane);
+      const float old_scale = *scale;
+      const uint32_t amax = __reduce_max_sync(0xffffffffu, max(finite_abs_max(v.x), finite_abs_max(v.y)));
+      const bool has_old = rg.start > row0;
+      const float s = grown_scale<kInt8>(amax, has_old, old_scale);
+      const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+      if (has_old && s != old_scale) {
+        const float ratio = old_scale / s;
+        for (int i = lane; i < (rg.start - row0) * 8; i += 32) {
+          uint4* q = reinterpret_cast<uint4*>(cache + static_cast<int64_t>(row0) * 128) + i;
+          *q = rescale8<kInt8>(*q, ratio);
+        }
+      }
+      reinterpret_cast<uint32_t*>(cache + static_cast<int64_t>(rg.start) * 128)[lane] =
+          pack8<kInt8>(bf_lo(v.x) * inv, bf_hi(v.x) * inv, bf_lo(v.y) * inv, bf_hi(v.y) * inv);
+      __syncwarp();
+      if (lane == 0) {
+        *scale = s;
+        if (kv == 0 && p.weights != nullptr) p.weights[unit * p.Smax + rg.start] = 0.0f;
+      }
+    }
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) p.seq_lens[b] = rg.end;
+}
+
+template <bool kInt8>
+cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
+  const dim3 grid((p.T - 1) / p.block + 2, 2 * p.Hkv, p.B);
+  switch (p.block) {
+    case 16: kv_append_kernel<kInt8, 1><<<grid, kAppendThreads, 0, stream>>>(p); break;
+    case 32: kv_append_kernel<kInt8, 2><<<grid, kAppendThreads, 0, stream>>>(p); break;
+    case 64: kv_append_kernel<kInt8, 4><<<grid, kAppendThreads, 0, stream>>>(p); break;
+    default: kv_append_kernel<kInt8, 8><<<grid, kAppendThreads, 0, stream>>>(p); break;
+  }
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  kv_advance_kernel<<<(p.B + 127) / 128, 128, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+// ---------------------------------------------------------------------------
+// evict: selection
+// ---------------------------------------------------------------------------
+// One cluster of 8 CTAs per (sequence, KV head), each CTA a contiguous eighth of the
+// rows and each warp a contiguous part of that.  The k-th largest weight of the
+// rows between the sink and the recent ones comes from a radix selection (digits
+// of 11, 11 and 10 bits of the order-preserving integer form; the CTAs' histograms
+// are added up through distributed shared memory), then a counting pass and an
+// emitting pass write the kept rows in order, rows equal to the threshold from the
+// lowest index on.  The weights are read five times, all but the first from L2.
+constexpr int kSelThreads = 512;
+constexpr int kSelCluster = 8;
+constexpr int kSelBins = 2048;
+constexpr int kSelWarps = kSelThreads / 32;
+
+// Order-preserving integer form of a weight; NaN below everything, -0 equal to +0.
+__device__ __forceinline__ uint32_t order_bits(float w) {
+  if (!(w == w)) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u ^ ((u >> 31) != 0u ? 0xFFFFFFFFu : 0x80000000u);
+}
+
+__global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThreads)
+    kv_select_kernel(const __grid_constant__ KvEvictParams p) {
+  __shared__ uint32_t hist[3][kSelBins];
+  __shared__ uint32_t warp_sum[kSelWarps];
+  __shared__ uint32_t found[2];
+  __shared__ uint32_t warp_gt[kSelWarps], warp_eq[kSelWarps];
+  __shared__ uint32_t cta_cnt[2];
+  cg::cluster_group cluster = cg::this_cluster();
+  const int64_t unit = blockIdx.x / kSelCluster;
+  const int rank = blockIdx.x % kSelCluster;
+  const int b = static_cast<int>(unit / p.Hkv);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int L = min(max(p.seq_lens[b], 0), p.Smax);
+  int32_t* slots = p.slots + unit * p.n;
+  if (L <= p.keep) {  // nothing to evict (the whole cluster agrees)
+    for (int i = rank * kSelThreads + tid; i < p.n; i += kSelCluster * kSelThreads) slots[i] = i < L ? i : -1;
+    return;
+  }
+  const float* w = p.src_weights + unit * p.Smax;
+  const int per_warp = ((L + kSelCluster * kSelWarps - 1) / (kSelCluster * kSelWarps) + 31) & ~31;
+  const int cta0 = rank * per_warp * kSelWarps;
+  const int cta1 = min(L, cta0 + per_warp * kSelWarps);
+  const int lo = p.sink, hi = L - p.recent;  // candidates (L > keep >= sink + recent)
+  const int c0 = max(cta0, lo), c1 = min(cta1, hi);
+  uint32_t need = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // < hi - lo
+  uint32_t thr = 0xFFFFFFFFu;  // need == 0: no weight is above it, and no equal one is taken
+  if (need > 0) {
+    for (int i = tid; i < 3 * kSelBins; i += kSelThreads) (&hist[0][0])[i] = 0u;
+    __syncthreads();
+    uint32_t pfx = 0;
+#pragma unroll
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
+      const uint32_t dmask = pass == 2 ? 1023u : 2047u;
+      const int up = pass == 0 ? 0 : (pass == 1 ? 21 : 10);  // the digits above: u >> up == pfx
+      for (int i = c0 + tid; i < c1; i += kSelThreads) {
+        const uint32_t u = order_bits(w[i]);
+        if (pass == 0 || (u >> up) == pfx) atomicAdd(&hist[pass][(u >> shift) & dmask], 1u);
+      }
+      cluster.sync();
+      // bins 4 tid .. 4 tid + 3 over the whole cluster, then the sum of the bins above them
+      uint4 mine = make_uint4(0, 0, 0, 0);
+#pragma unroll
+      for (int r = 0; r < kSelCluster; ++r) {
+        const uint4 h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[pass][0], r))[tid];
+        mine.x += h.x;
+        mine.y += h.y;
+        mine.z += h.z;
+        mine.w += h.w;
+      }
+      const uint32_t total = mine.x + mine.y + mine.z + mine.w;
+      uint32_t suffix = total;  // over this lane and the lanes above it
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t t = __shfl_down_sync(0xffffffffu, suffix, o);
+        if (lane + o < 32) suffix += t;
+      }
+      if (lane == 0) warp_sum[warp] = suffix;
+      __syncthreads();
+      uint32_t above = suffix - total;
+      for (int k = warp + 1; k < kSelWarps; ++k) above += warp_sum[k];
+      if (above < need && above + total >= need) {  // exactly one thread
+        const uint32_t bin[4] = {mine.x, mine.y, mine.z, mine.w};
+        int d = 3;
+        while (d > 0 && above + bin[d] < need) above += bin[d--];
+        found[0] = static_cast<uint32_t>(4 * tid + d);
+        found[1] = need - above;
+      }
+      __syncthreads();
+      pfx = pass == 2 ? (pfx << 10) | found[0] : (pfx << 11) | found[0];
+      need = found[1];
+      __syncthreads();
+    }
+    thr = pfx;
+  }
+  // rows above the threshold (and the sink and recent rows) and rows equal to it, per warp
+  const int w0 = cta0 + warp * per_warp, w1 = min(cta1, w0 + per_warp);
+  auto classify = [&](int i, bool& gt, bool& eq) {
+    gt = eq = false;
+    if (i < w1) {
+      if (i < lo || i >= hi) {
+        gt = true;
+      } else {
+        const uint32_t u = order_bits(w[i]);
+        gt = u > thr;
+        eq = u == thr;
+      }
+    }
+  };
+  uint32_t ngt = 0, neq = 0;
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    bool gt, eq;
+    classify(i0 + lane, gt, eq);
+    ngt += __popc(__ballot_sync(0xffffffffu, gt));
+    neq += __popc(__ballot_sync(0xffffffffu, eq));
+  }
+  if (lane == 0) {
+    warp_gt[warp] = ngt;
+    warp_eq[warp] = neq;
+  }
+  __syncthreads();
+  uint32_t gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
+  for (int k = 0; k < kSelWarps; ++k) {
+    if (k < warp) {
+      gt_before += warp_gt[k];
+      eq_before += warp_eq[k];
+    }
+    gt_all += warp_gt[k];
+    eq_all += warp_eq[k];
+  }
+  if (tid == 0) {
+    cta_cnt[0] = gt_all;
+    cta_cnt[1] = eq_all;
+  }
+  cluster.sync();
+  for (int r = 0; r < rank; ++r) {
+    const uint32_t* other = cluster.map_shared_rank(&cta_cnt[0], r);
+    gt_before += other[0];
+    eq_before += other[1];
+  }
+  cluster.sync();  // the counts (and histograms) of a CTA are read no more: it may exit
+  const uint32_t below = (1u << lane) - 1u;
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    bool gt, eq;
+    classify(i0 + lane, gt, eq);
+    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
+    const uint32_t er = eq_before + __popc(be & below);
+    if (gt || (eq && er < need)) {
+      const uint32_t at = gt_before + __popc(bg & below) + min(er, need);
+      slots[at] = i0 + lane;
+    }
+    gt_before += __popc(bg);
+    eq_before += __popc(be);
+  }
+}
+
+// ---------------------------------------------------------------------------
+// evict: move
+// ---------------------------------------------------------------------------
+// A CTA gathers 128 destination rows of one (sequence, KV head), K and V, into
+// registers (8 x 16 bytes per thread), then rounds them to their destination
+// block's scale (the largest of its rows' scales: rows of that scale keep their
+// bytes) and stores them.  HBM-bound: each kept row is read and written once.
+//   Out of place: one CTA per 128 rows.
+//   In place: a cluster of 8 CTAs walks over the rows of its (sequence, KV head)
+//   1024 at a time; all eight have read their rows before any of them writes.  A
+//   kept row's source lies at or behind its destination, so a later step's sources
+//   (rows and scales) are never behind an earlier step's stores.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 128;
+constexpr int kMoveCluster = 8;
+
+template <bool kInt8, bool kInPlace>
+__device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, int base, bool sync_cluster) {
+  __shared__ int slot_sh[kMoveRows];
+  __shared__ float scale_sh[2][kMoveRows];
+  __shared__ float warp_max[2][kMoveRows / 32];
+  const int tid = threadIdx.x;
+  // -1: no row, here or further on
+  int slot = -1;
+  float s[2] = {0.0f, 0.0f}, weight = 0.0f;
+  bool moved = false;
+  if (tid < kMoveRows) {
+    const int row = base + tid;
+    if (row < p.n) slot = p.slots[unit * p.n + row];
+    moved = slot != row && slot >= 0;
+    if (slot >= 0) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) s[kv] = p.src_scale[kv][unit * p.nblk + slot / p.block];
+      weight = p.src_weights[unit * p.Smax + slot];
+    }
+    slot_sh[tid] = slot;
+  }
+  const bool work = __syncthreads_or(kInPlace ? moved : slot >= 0) != 0;
+  uint4 v[8];
+  if (work) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 32 * (i & 3) + (tid >> 3);
+      const int src = slot_sh[r];
+      v[i] = make_uint4(0, 0, 0, 0);
+      if (src >= 0)
+        v[i] = *reinterpret_cast<const uint4*>(p.src[i >> 2] + (unit * p.Smax + src) * 128 + 16 * (tid & 7));
+    }
+    // destination scale of each row: the maximum over its block
+    if (tid < kMoveRows) {
+      float m[2] = {s[0], s[1]};
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1)
+          if (o < p.block) m[kv] = fmaxf(m[kv], __shfl_xor_sync(0xffffffffu, m[kv], o));
+        if ((tid & 31) == 0) warp_max[kv][tid >> 5] = m[kv];
+      }
+      scale_sh[0][tid] = m[0];
+      scale_sh[1][tid] = m[1];
+    }
+    __syncthreads();
+    float d[2] = {0.0f, 0.0f};
+    if (tid < kMoveRows) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) {
+        d[kv] = scale_sh[kv][tid];
+        if (p.block > 32) {
+          const int per = p.block / 32, first = (tid >> 5) / per * per;
+          for (int k = 0; k < per; ++k) d[kv] = fmaxf(d[kv], warp_max[kv][first + k]);
+        }
+      }
+    }
+    __syncthreads();
+    if (tid < kMoveRows) {
+#pragma unroll
+      for (int kv = 0; kv < 2; ++kv) scale_sh[kv][tid] = s[kv] == d[kv] ? 1.0f : s[kv] / d[kv];
+    }
+    __syncthreads();
+    if (kInPlace && sync_cluster) cg::this_cluster().sync();
+    if (tid < kMoveRows && slot >= 0) {
+      const int row = base + tid;
+      p.dst_weights[unit * p.Smax_dst + row] = weight;
+      if (tid % p.block == 0) {
+#pragma unroll
+        for (int kv = 0; kv < 2; ++kv) p.dst_scale[kv][unit * p.nblk_dst + row / p.block] = d[kv];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int r = 32 * (i & 3) + (tid >> 3);
+      if (slot_sh[r] < 0) continue;
+      const float ratio = scale_sh[i >> 2][r];
+      const uint4 o = ratio == 1.0f ? v[i] : rescale8<kInt8>(v[i], ratio);
+      *reinterpret_cast<uint4*>(p.dst[i >> 2] + (unit * p.Smax_dst + base + r) * 128 + 16 * (tid & 7)) = o;
+    }
+  } else if (kInPlace && sync_cluster) {
+    cg::this_cluster().sync();
+  }
+}
+
+__device__ __forceinline__ void write_kept_length(const KvEvictParams& p, int64_t unit) {
+  if (unit % p.Hkv == 0 && threadIdx.x == 0) {
+    const int b = static_cast<int>(unit / p.Hkv);
+    p.dst_lens[b] = min(min(max(p.seq_lens[b], 0), p.Smax), p.keep);
+  }
+}
+
+template <bool kInt8>
+__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ KvEvictParams p, int tiles) {
+  const int64_t unit = blockIdx.x / tiles;
+  const int tile = blockIdx.x % tiles;
+  move_rows<kInt8, false>(p, unit, tile * kMoveRows, false);
+  if (tile == 0) write_kept_length(p, unit);
+}
+
+template <bool kInt8>
+__global__ void __cluster_dims__(kMoveCluster, 1, 1) __launch_bounds__(kMoveThreads)
+    kv_move_in_place_kernel(const __grid_constant__ KvEvictParams p) {
+  const int64_t unit = blockIdx.x / kMoveCluster;
+  const int rank = blockIdx.x % kMoveCluster;
+  for (int step = 0; step < p.n; step += kMoveCluster * kMoveRows) {
+    move_rows<kInt8, true>(p, unit, step + rank * kMoveRows, true);
+    __syncthreads();
+  }
+  if (rank == 0) write_kept_length(p, unit);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_append(const KvAppendParams& p, bool int8, cudaStream_t stream) {
+  if (p.T == 1) {
+    const int threads = 32 * (2 * p.Hkv < 32 ? 2 * p.Hkv : 32);
+    if (int8) {
+      kv_append_token_kernel<true><<<p.B, threads, 0, stream>>>(p);
+    } else {
+      kv_append_token_kernel<false><<<p.B, threads, 0, stream>>>(p);
+    }
+    return cudaGetLastError();
+  }
+  return int8 ? append_rows<true>(p, stream) : append_rows<false>(p, stream);
+}
+
+cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream) {
+  const int units = p.B * p.Hkv;
+  kv_select_kernel<<<units * kSelCluster, kSelThreads, 0, stream>>>(p);
+  cudaError_t e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  if (in_place) {
+    if (int8) {
+      kv_move_in_place_kernel<true><<<units * kMoveCluster, kMoveThreads, 0, stream>>>(p);
+    } else {
+      kv_move_in_place_kernel<false><<<units * kMoveCluster, kMoveThreads, 0, stream>>>(p);
+    }
+  } else {
+    const int tiles = (p.n + kMoveRows - 1) / kMoveRows;
+    if (int8) {
+      kv_move_kernel<true><<<units * tiles, kMoveThreads, 0, stream>>>(p, tiles);
+    } else {
+      kv_move_kernel<false><<<units * tiles, kMoveThreads, 0, stream>>>(p, tiles);
+    }
+  }
+  return cudaGetLastError();
+}
+
+}  // namespace swa

@@ -1,0 +1,77 @@
+// Block-scaled 8-bit KV cache: parameters shared by its kernels and entry points.
+//
+// K and V are [B, Hkv, Smax, 128] bytes (e4m3 or int8): the rows of one KV head lie
+// together, so 128 keys are one contiguous 16 KB tile (the token-major layout of
+// the BF16 cache would make it 128 pieces of 128 bytes).  Every block of `block`
+// rows (16, 32, 64 or 128) of a head has one FP32 scale for K and one for V,
+// [B, Hkv, nblk], nblk = ceil(Smax / block): value = byte * scale.
+#pragma once
+
+#include <cstdint>
+#include <cuda.h>
+#include <cuda_runtime.h>
+#include <cuda_bf16.h>
+
+namespace swa {
+
+struct KvAppendParams {
+  const __nv_bfloat16* x[2];  // new K, V rows: element (b, t, g, d) at b * sb + t * st + g * sh + d
+  int64_t sb[2], st[2], sh[2];
+  uint8_t* cache[2];          // [B, Hkv, Smax, 128]
+  float* scale[2];            // [B, Hkv, nblk]
+  float* weights;             // [B, Hkv, Smax] or null; new rows start at 0
+  const int32_t* start;       // [B] rows already cached (may be seq_lens)
+  const int32_t* new_lens;    // [B] new rows of each sequence, or null: T
+  int32_t* seq_lens;          // [B] written: rows cached after the call
+  int B, T, Hkv, Smax, nblk, block;
+};
+cudaError_t launch_kv_append(const KvAppendParams& p, bool int8, cudaStream_t stream);
+
+struct KvEvictParams {
+  const uint8_t* src[2];      // K, V caches [B, Hkv, Smax, 128]
+  const float* src_scale[2];  // [B, Hkv, nblk]
+  const float* src_weights;   // [B, Hkv, Smax]
+  uint8_t* dst[2];            // [B, Hkv, Smax_dst, 128]; in place: the same pointers
+  float* dst_scale[2];        // [B, Hkv, nblk_dst]
+  float* dst_weights;         // [B, Hkv, Smax_dst]
+  const int32_t* seq_lens;    // [B]
+  int32_t* dst_lens;          // [B] written: min(length, keep); in place: seq_lens
+  int32_t* slots;             // [B, Hkv, n] written: source row of each kept row, -1 past the count
+  int B, Hkv, Smax, Smax_dst, nblk, nblk_dst, block, n, keep, sink, recent;
+};
+cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream);
+
+// Decode over the cache.  The (sequence, KV head, head block) units' legal keys are
+// cut into tiles of 128 keys, all tiles of the batch are laid end to end in the order
+// (sequence, KV head, head block, tile), and each of the `ctas` CTAs takes `per` =
+// ceil(tiles / ctas) consecutive ones.  A CTA's share of one unit is a segment; its
+// partial result lies in slot unit + cta (both grow along the order and each new
+// segment moves one of them, so slots are distinct).
+struct __align__(64) KvDecodeParams {
+  CUtensorMap map[2];         // K, V bytes: 3-D {128, Smax, B * Hkv}, box {128, 128, 1}, 128B swizzle
+  const __nv_bfloat16* q;     // element (b, h, d) at b * q_sb + h * q_sh + d
+  int64_t q_sb, q_sh;
+  const float* scale[2];      // [B, Hkv, nblk]
+  const int32_t* seq_lens;    // [B] cached keys, the new token's included
+  const uint8_t* route;       // [B] non-zero = full attention
+  __nv_bfloat16* out;         // [B, Hq, 128]
+  float* lse;                 // [B, Hq]
+  float* weights;             // [B, Hkv, Smax] added to, or null
+  // workspace
+  int32_t* cum;               // [B + 1] tiles of one head of the sequences before b
+  int32_t* cta_status;        // [ctas]
+  int32_t* status;
+  float* part_ml;             // [slots, heads, 2] maximum and sum of each partial row
+  float* part_o;              // [slots, heads, 128]
+  float* scores;              // [tiles, heads, 128] log2-domain scores (with weights)
+  int B, Smax, Hq, Hkv, r, nblk, block_shift, window;
+  int heads;                  // query heads of a head block: 4 or 8
+  int nhb;                    // head blocks per KV head
+  int ctas;
+  float scale_log2;
+};
+cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream);
+// Resident CTAs of the decode kernel per SM (what its shared memory allows).
+constexpr int kKvDecodeCtasPerSm = 2;
+
+}  // namespace swa

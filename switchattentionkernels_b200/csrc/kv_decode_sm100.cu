@@ -1,0 +1,758 @@
+// Decode attention over the block-scaled 8-bit KV cache on B200 (sm_100a): one query
+// token per sequence attends to its cached keys [lo, L), lo = 0 (full) or
+// max(0, L - window), with value = byte * scale[block of the key]:
+//   s_hk = scale_log2 * ks_k * (q_h . k8_k)        (log2 domain)
+//   O_h  = sum_k 2^(s_hk - lse_h) vs_k v8_k,  lse_h = log2 sum_k 2^s_hk
+//   weights_k += sum over the heads h of the group of 2^(s_hk - lse_h)   (optional)
+//
+// HBM-bound: 256 bytes per (key, KV head).  The bytes go from TMA to the tensor cores
+// as they are, with no conversion in between: the 8-bit operand is the M side,
+//   S^T [128 keys x N]  = K tile [128 x 128 B] (K-major)  .  Qp^T
+//   O^T [128 dims x N]  = V tile^T (MN-major)             .  Pp^T
+// and the few query heads the N side.  Q and P, which have more than 8 bits, are cut
+// into three 8-bit parts, a column each: e4m3 parts of 4 significant bits (kind::f8f6f4,
+// 12 bits in all: BF16 q exactly, P as FP16) or signed-byte digits (kind::i8, 23 bits and
+// exact INT32 sums).  The parts' results are added up in FP32.
+//
+// Roles of a CTA (192 threads): warps 0-3 softmax, warp 4 TMA producer, warp 5 MMA issuer.
+// A softmax thread owns one key of a tile (TMEM lane) when it reads S^T, and one of the
+// 128 dims when it reads O^T: O is kept in its registers, one value per head, and each
+// tile's O^T is added with the tile's own factor, so P is taken relative to the tile's
+// maximum (never above 1) and V relative to the tile's largest V scale.
+#include <cuda_fp16.h>
+
+#include "kv_cache.h"
+#include "mma_sync.cuh"
+#include "sm100.cuh"
+#include "swattn_internal.h"
+
+namespace swa {
+
+namespace {
+
+constexpr int kTile = 128;                 // keys of a tile
+constexpr int kTileBytes = kTile * 128;
+constexpr int kStages = 3;                 // K tiles and V tiles in flight
+constexpr int kThreads = 192;
+constexpr int kParts = 3;
+constexpr float kE4m3Step = 16.0f;         // weight of an e4m3 part against the next
+constexpr float kInt8One = 8323072.0f;     // 127 * 65536: 1.0 as three signed-byte digits
+
+template <int kHeads>
+struct KvSmem {
+  static constexpr int cols = kHeads <= 4 ? 16 : 32;  // N: parts x heads, padded
+  static constexpr uint32_t k = 0;
+  static constexpr uint32_t v = k + kStages * kTileBytes;
+  static constexpr uint32_t q = v + kStages * kTileBytes;          // [cols][128 B]
+  static constexpr uint32_t p = q + cols * 128;                    // 2 x [cols][128 B]
+  static constexpr uint32_t red = p + 2 * cols * 128;              // [2][4 warps][12] floats
+  static constexpr uint32_t lred = red + 2 * 4 * 12 * 4;           // [2][4 warps][8] floats
+  static constexpr uint32_t qf = lred + 2 * 4 * 8 * 4;             // [8] floats
+  static constexpr uint32_t bars = qf + 32;
+  static constexpr uint32_t misc = bars + 24 * 8;                  // tmem holder, abort flag, start of the share
+  static constexpr uint32_t total = misc + 64;
+  static constexpr uint32_t bytes = total + 1024;
+};
+
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag));
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+struct KeyRange {
+  int lo, hi;
+};
+__device__ __forceinline__ KeyRange key_range(const KvDecodeParams& p, int b) {
+  const int L = min(max(p.seq_lens[b], 0), p.Smax);
+  return KeyRange{p.route[b] != 0 ? 0 : max(0, L - p.window), L};
+}
+__device__ __forceinline__ int seq_tiles(const KvDecodeParams& p, int b) {
+  const KeyRange r = key_range(p, b);
+  return (r.hi - r.lo + kTile - 1) / kTile;
+}
+
+// A CTA's share of the tiles, segment by segment.
+struct Segments {
+  int b, u, off, left;  // sequence, unit in it (KV head x head block), first tile in the unit, tiles left
+  // current segment
+  int lo, hi, first, n, all;  // legal keys; first tile, tiles; tiles of the unit
+  __device__ __forceinline__ bool next(const KvDecodeParams& p) {
+    if (left <= 0) return false;
+    for (;; ++b) {  // (only sequences without a key are skipped)
+      const KeyRange r = key_range(p, b);
+      all = (r.hi - r.lo + kTile - 1) / kTile;
+      lo = r.lo;
+      hi = r.hi;
+      if (all > 0) break;
+    }
+    cur_b = b;
+    cur_u = u;
+    first = off;
+    n = min(all - off, left);
+    left -= n;
+    off += n;
+    if (off == all) {
+      off = 0;
+      if (++u == p.Hkv * p.nhb) {
+        u = 0;
+        ++b;
+      }
+    }
+    return true;
+  }
+  int cur_b, cur_u;
+};
+
+__device__ __forceinline__ float pow2_at_least_448th(float a) {  // smallest 2^e with 448 * 2^e >= a
+  const uint32_t bits = __float_as_uint(a);
+  const int e = static_cast<int>(bits >> 23) - 127 - 8 + ((bits & 0x7FFFFFu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(static_cast<uint32_t>(min(max(e, -126), 127) + 127) << 23);
+}
+
+__device__ __forceinline__ uint16_t f16x2_to_e4m3x2(uint32_t h) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f16x2 %0, %1;" : "=h"(r) : "r"(h));
+  return r;
+}
+__device__ __forceinline__ __half2 e4m3x2_to_f16x2(uint16_t v) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(r) : "h"(v));
+  return *reinterpret_cast<__half2*>(&r);
+}
+
+// Two values (|x| <= 448) as three e4m3 parts each: x = p0 + p1 / 16 + p2 / 256, the
+// parts' pairs as bytes (low byte: first value).  e4m3 has 4 significant bits, so the
+// rest left by a part is at most 1/16 of its value's binade and 16 times it is in
+// range again: together the parts hold the 11 bits of an FP16 x, down to steps of 2^-17
+// (the last part's smallest, 2^-9 / 256).
+__device__ __forceinline__ void split_e4m3(__half2 x, uint16_t* part) {
+  part[0] = f16x2_to_e4m3x2(*reinterpret_cast<uint32_t*>(&x));
+  const __half2 r1 = __hsub2(x, e4m3x2_to_f16x2(part[0]));
+  __half2 y = __hmul2(r1, __float2half2_rn(kE4m3Step));
+  part[1] = f16x2_to_e4m3x2(*reinterpret_cast<uint32_t*>(&y));
+  y = __hmul2(__hsub2(y, e4m3x2_to_f16x2(part[1])), __float2half2_rn(kE4m3Step));
+  part[2] = f16x2_to_e4m3x2(*reinterpret_cast<uint32_t*>(&y));
+}
+
+// A value in [-1, 1] in steps of 1 / 8323072 as three signed bytes (byte 2 the highest).
+__device__ __forceinline__ uint32_t split_int8(float x) {
+  return static_cast<uint32_t>(__float2int_rn(x * kInt8One) + 0x008080) ^ 0x008080u;
+}
+
+// Sum of the parts' results of head h (accumulator columns part * kHeads + h).
+template <bool kInt8, int kHeads>
+__device__ __forceinline__ float join_parts(const uint32_t* c, int h) {
+  if constexpr (kInt8) {
+    return fmaf(static_cast<float>(static_cast<int>(c[h])), 65536.0f,
+                fmaf(static_cast<float>(static_cast<int>(c[kHeads + h])), 256.0f,
+                     static_cast<float>(static_cast<int>(c[2 * kHeads + h]))));
+  } else {
+    return fmaf(__uint_as_float(c[2 * kHeads + h]), 1.0f / (kE4m3Step * kE4m3Step),
+                fmaf(__uint_as_float(c[kHeads + h]), 1.0f / kE4m3Step, __uint_as_float(c[h])));
+  }
+}
+
+template <int kCols>
+__device__ __forceinline__ void tmem_ld_cols(uint32_t addr, uint32_t* c) {
+  if constexpr (kCols == 16) {
+    tmem_ld_x16(addr, c);
+    tmem_ld_wait();
+    reg_fence16(c);
+  } else {
+    tmem_ld_x32(addr, c);
+    tmem_ld_wait();
+    reg_fence32(c);
+  }
+}
+
+// kWeights: also stores every legal key's scores for the second kernel.
+template <bool kInt8, int kHeads, bool kWeights>
+__global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
+    kv_decode_kernel(const __grid_constant__ KvDecodeParams p) {
+  using Sm = KvSmem<kHeads>;
+  constexpr int kCols = Sm::cols;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem =
+      reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~static_cast<uintptr_t>(1023));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + Sm::bars);
+  uint64_t* k_empty = k_full + kStages;
+  uint64_t* v_full = k_empty + kStages;
+  uint64_t* v_empty = v_full + kStages;
+  uint64_t* s_full = v_empty + kStages;  // [2] scores of a tile in TMEM
+  uint64_t* p_full = s_full + 2;         // [2] P of a tile in shared memory (and its scores read)
+  uint64_t* o_full = p_full + 2;         // [2] O^T of a tile in TMEM
+  uint64_t* red_full = o_full + 2;       // [2] the four warps' maxima of a tile
+  uint64_t* q_full = red_full + 2;       // Q parts of a segment
+  uint64_t* l_full = q_full + 1;         // the four warps' row sums of a segment
+  uint64_t* done = l_full + 1;
+  static_assert(4 * kStages + 4 * 2 + 3 <= 24, "barrier space");
+  uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + Sm::misc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::misc + 4);
+  int* share = reinterpret_cast<int*>(smem + Sm::misc + 8);  // of this CTA: sequence, unit, tile in it, tiles, first tile
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta = blockIdx.x;
+  const int units = p.Hkv * p.nhb;  // units of a sequence
+
+  if (tid == 0) {
+    for (int s = 0; s < kStages; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 128);
+      mbar_init(&o_full[i], 1);
+      mbar_init(&red_full[i], 4);
+    }
+    mbar_init(q_full, 128);
+    mbar_init(l_full, 4);
+    mbar_init(done, 1);
+    *abort_flag = 0;
+    share[3] = 0;
+    fence_barrier_init();
+  }
+  // unused columns of Q and P are zero
+  for (int i = tid; i < 3 * kCols * 8; i += kThreads)
+    reinterpret_cast<uint4*>(smem + Sm::q)[i] = make_uint4(0, 0, 0, 0);
+  fence_proxy_async_smem();
+  {
+    // this CTA's share: thread t sums the tiles of a run of sequences, then a scan over the threads
+    int* scan = reinterpret_cast<int*>(smem + Sm::red);
+    const int run = (p.B + kThreads - 1) / kThreads;
+    const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
+    int sum = 0;
+    for (int b = b0; b < b1; ++b) sum += seq_tiles(p, b);
+    int incl = sum;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += t;
+    }
+    if (lane == 31) scan[warp] = incl;
+    __syncthreads();
+    int before = incl - sum, total = 0;
+    for (int w = 0; w < kThreads / 32; ++w) {
+      if (w < warp) before += scan[w];
+      total += scan[w];
+    }
+    if (cta == 0) {
+      int c = before;
+      for (int b = b0; b < b1; ++b) {
+        p.cum[b] = c;
+        c += seq_tiles(p, b);
+      }
+      if (tid == 0) p.cum[p.B] = total;
+    }
+    const int tiles = total * units;
+    const int per = (tiles + p.ctas - 1) / p.ctas;
+    const int t0 = cta * per, t1 = min(tiles, t0 + per);
+    if (t0 < t1 && t0 >= before * units && t0 < (before + sum) * units) {  // exactly one thread
+      int b = b0, c = before * units;
+      for (;; ++b) {
+        const int nb = seq_tiles(p, b) * units;
+        if (t0 < c + nb) break;
+        c += nb;
+      }
+      const int nb = seq_tiles(p, b);
+      share[0] = b;
+      share[1] = (t0 - c) / nb;
+      share[2] = (t0 - c) % nb;
+      share[3] = t1 - t0;
+      share[4] = t0;
+    }
+  }
+  if (warp == 5) {
+    __syncwarp();
+    tmem_alloc(tmem_holder, 4 * kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_holder;  // S: columns 0 and kCols, O: 2 kCols and 3 kCols
+  const int ntiles = share[3];
+  Segments seg{};
+  seg.b = share[0];
+  seg.u = share[1];
+  seg.off = share[2];
+  seg.left = ntiles;
+
+  if (warp == 4) {
+    // ------------------------------------------------------------ TMA producer
+    if (lane == 0 && ntiles > 0) {
+      tma_prefetch_desc(&p.map[0]);
+      tma_prefetch_desc(&p.map[1]);
+      int it = 0, iv = 0;  // K and V tiles issued
+      bool ok = true;
+      while (ok && seg.next(p)) {
+        const int row = seg.cur_b * p.Hkv + seg.cur_u / p.nhb;
+        for (int i = 0; i < seg.n; ++i) {
+          const int s = it % kStages;
+          const uint32_t ph = ((it / kStages) & 1) ^ 1;
+          const int key0 = seg.lo + (seg.first + i) * kTile;
+          if (!(ok = mbar_wait(&k_empty[s], ph, abort_flag))) break;
+          mbar_arrive_expect_tx(&k_full[s], kTileBytes);
+          tma_load_3d(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row);
+          ++it;
+          if (!(ok = mbar_wait(&v_empty[s], ph, abort_flag))) break;
+          mbar_arrive_expect_tx(&v_full[s], kTileBytes);
+          tma_load_3d(smem + Sm::v + s * kTileBytes, &p.map[1], &v_full[s], 0, key0, row);
+          ++iv;
+        }
+      }
+      if (*abort_flag) {
+        // let the loads already issued land before the CTA's shared memory is released
+        volatile int dummy = 0;
+        for (int t = max(0, it - kStages); t < it; ++t) mbar_wait(&k_full[t % kStages], (t / kStages) & 1, &dummy);
+        for (int t = max(0, iv - kStages); t < iv; ++t) mbar_wait(&v_full[t % kStages], (t / kStages) & 1, &dummy);
+      }
+    }
+  } else if (warp == 5) {
+    // ------------------------------------------------------------ MMA issuer
+    constexpr uint32_t idesc_s = make_idesc_8bit(kInt8, 128, kCols, false, false);
+    constexpr uint32_t idesc_o = make_idesc_8bit(kInt8, 128, kCols, true, false);
+    const uint64_t q_desc = make_smem_desc_sw128(smem_u32(smem + Sm::q), 16, 1024);
+    bool ok = true;
+    int pv = 0;  // tiles whose PV product has been issued
+    auto issue_pv = [&]() {
+      const int s = pv % kStages;
+      if (!warp_wait(&v_full[s], (pv / kStages) & 1, abort_flag)) return false;
+      if (!warp_wait(&p_full[pv & 1], (pv >> 1) & 1, abort_flag)) return false;
+      tc_fence_after();
+      const uint64_t v_desc = make_smem_desc_sw128(smem_u32(smem + Sm::v + s * kTileBytes), kTileBytes, 1024);
+      const uint64_t p_desc = make_smem_desc_sw128(smem_u32(smem + Sm::p + (pv & 1) * kCols * 128), 16, 1024);
+      umma8_ss_k128_warp<kInt8>(tmem + (2 + (pv & 1)) * kCols, v_desc, p_desc, 32 * 128 / 16, 2, idesc_o);
+      tc_commit_warp(&o_full[pv & 1]);
+      tc_commit_warp(&v_empty[s]);
+      ++pv;
+      return true;
+    };
+    int it = 0, nseg = 0;
+    while (ok && seg.next(p)) {
+      // the softmax warps write a segment's Q after they have taken the last O of the one before
+      while (ok && pv < it) ok = issue_pv();
+      ok = ok && warp_wait(q_full, nseg & 1, abort_flag);
+      ++nseg;
+      for (int i = 0; i < seg.n && ok; ++i, ++it) {
+        const int s = it % kStages;
+        if (!(ok = warp_wait(&k_full[s], (it / kStages) & 1, abort_flag))) break;
+        tc_fence_after();
+        // score buffer it & 1 was read before P of tile it - 2, whose product is issued
+        const uint64_t k_desc = make_smem_desc_sw128(smem_u32(smem + Sm::k + s * kTileBytes), 16, 1024);
+        umma8_ss_k128_warp<kInt8>(tmem + (it & 1) * kCols, k_desc, q_desc, 2, 2, idesc_s);
+        tc_commit_warp(&s_full[it & 1]);
+        tc_commit_warp(&k_empty[s]);
+        while (ok && pv < it) ok = issue_pv();
+      }
+    }
+    while (ok && pv < it) ok = issue_pv();
+    tc_commit_warp(done);  // every MMA issued, before the CTA frees its tensor memory
+    volatile int dummy = 0;
+    mbar_wait(done, 0, &dummy);
+  } else {
+    // ------------------------------------------------------------ softmax warps
+    const uint32_t lane_off = static_cast<uint32_t>(32 * warp) << 16;
+    float* red = reinterpret_cast<float*>(smem + Sm::red);
+    float* lred = reinterpret_cast<float*>(smem + Sm::lred);
+    float* qf = reinterpret_cast<float*>(smem + Sm::qf);
+    bool ok = true;
+    int it = 0, nseg = 0;
+    int64_t tile_id = share[4];  // of the whole batch
+    while (ok && seg.next(p)) {
+      const int g = seg.cur_u / p.nhb, hb = seg.cur_u % p.nhb;
+      const int head0 = g * p.r + hb * kHeads;           // first query head of the block
+      const int nh = min(kHeads, p.r - hb * kHeads);     // heads that exist
+      // Q parts: 16 threads per head, 8 dims each
+      {
+        const int h = tid >> 4, c = tid & 15;
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (h < nh)
+          w = *reinterpret_cast<const uint4*>(p.q + seg.cur_b * p.q_sb + (head0 + h) * p.q_sh + 8 * c);
+        const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+        float x[8];
+        float amax = 0.0f;
+        bool finite = true;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          x[i] = __uint_as_float((i & 1) ? (wd[i >> 1] & 0xFFFF0000u) : (wd[i >> 1] << 16));
+          finite = finite && fabsf(x[i]) < INFINITY;
+          amax = fmaxf(amax, fabsf(x[i]));
+        }
+#pragma unroll
+        for (int o = 1; o < 16; o <<= 1) {
+          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+          finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, o) != 0 && finite;
+        }
+        if (h < kHeads) {
+          uint32_t lo[kParts], hi[kParts];  // bytes of dims 0-3 and 4-7
+          float unit;                       // value of one step of the parts' sum
+          if constexpr (kInt8) {
+            unit = amax / kInt8One;
+            const float inv = (amax > 0.0f && finite) ? 1.0f / amax : 0.0f;
+#pragma unroll
+            for (int pt = 0; pt < kParts; ++pt) lo[pt] = hi[pt] = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t v = split_int8(x[i] * inv);
+#pragma unroll
+              for (int pt = 0; pt < kParts; ++pt) {
+                const uint32_t byte = (v >> (16 - 8 * pt)) & 0xFFu;
+                if (i < 4) lo[pt] |= byte << (8 * i); else hi[pt] |= byte << (8 * (i - 4));
+              }
+            }
+          } else {
+            unit = amax > 0.0f ? pow2_at_least_448th(amax) : 1.0f;  // a power of two: x / unit is exact
+            const float inv = finite ? 1.0f / unit : 0.0f;
+            uint16_t pr[4][kParts];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) split_e4m3(__floats2half2_rn(x[2 * i] * inv, x[2 * i + 1] * inv), pr[i]);
+#pragma unroll
+            for (int pt = 0; pt < kParts; ++pt) {
+              lo[pt] = pr[0][pt] | (static_cast<uint32_t>(pr[1][pt]) << 16);
+              hi[pt] = pr[2][pt] | (static_cast<uint32_t>(pr[3][pt]) << 16);
+            }
+          }
+#pragma unroll
+          for (int pt = 0; pt < kParts; ++pt) {
+            const int n = pt * kHeads + h;
+            *reinterpret_cast<uint2*>(smem + Sm::q + n * 128 + (((c >> 1) ^ (n & 7)) << 4) + 8 * (c & 1)) =
+                make_uint2(lo[pt], hi[pt]);
+          }
+          // a query with an infinity or NaN has no finite score: NaN all through
+          if (c == 0) qf[h] = finite ? p.scale_log2 * unit : __uint_as_float(0x7FC00000u);
+        }
+        fence_proxy_async_smem();
+        mbar_arrive(q_full);
+      }
+      if (!(ok = warp_wait(q_full, nseg & 1, abort_flag))) break;
+      float f[kHeads], m[kHeads], l[kHeads], o[kHeads], alpha[kHeads], beta[kHeads];
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        f[h] = qf[h];
+        m[h] = -INFINITY;
+        l[h] = o[h] = alpha[h] = beta[h] = 0.0f;
+      }
+      const int64_t kvrow = static_cast<int64_t>(seg.cur_b) * p.Hkv + g;
+      const float* ks_row = p.scale[0] + kvrow * p.nblk;
+      const float* vs_row = p.scale[1] + kvrow * p.nblk;
+      const int key_first = seg.lo + seg.first * kTile + tid;
+      int blk = min(key_first, seg.hi - 1) >> p.block_shift;
+      float ks_next = ks_row[blk], vs_next = vs_row[blk];
+      // adds O^T of tile t (relative to that tile's maximum and V scale)
+      auto take_o = [&](int t) {
+        if (!warp_wait(&o_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
+        tc_fence_after();
+        uint32_t c[kCols];
+        tmem_ld_cols<kCols>(tmem + (2 + (t & 1)) * kCols + lane_off, c);
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) o[h] = fmaf(join_parts<kInt8, kHeads>(c, h), beta[h], o[h] * alpha[h]);
+        return true;
+      };
+      for (int i = 0; i < seg.n && ok; ++i, ++it) {
+        const int key0 = seg.lo + (seg.first + i) * kTile;
+        const bool legal = key0 + tid < seg.hi;
+        const float ks = ks_next, vs = legal ? vs_next : 0.0f;
+        if (i + 1 < seg.n) {
+          blk = min(key0 + kTile + tid, seg.hi - 1) >> p.block_shift;
+          ks_next = ks_row[blk];
+          vs_next = vs_row[blk];
+        }
+        const int buf = it & 1;
+        if (!(ok = warp_wait(&s_full[buf], (it >> 1) & 1, abort_flag))) break;
+        tc_fence_after();
+        float s[kHeads];
+        {
+          uint32_t c[kCols];
+          tmem_ld_cols<kCols>(tmem + buf * kCols + lane_off, c);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) s[h] = legal ? join_parts<kInt8, kHeads>(c, h) * (f[h] * ks) : -INFINITY;
+        }
+        if constexpr (kWeights) {
+          float* dst = p.scores + tile_id * kHeads * kTile + tid;
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) dst[h * kTile] = s[h];
+          ++tile_id;
+        }
+        // maxima of the tile over its keys
+        float* rb = red + buf * 48;
+        float mt[kHeads], vref;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) mt[h] = warp_max(s[h]);
+        vref = warp_max(vs);
+        if (lane == 0) {
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) rb[warp * 12 + h] = mt[h];
+          rb[warp * 12 + kHeads] = vref;
+          mbar_arrive(&red_full[buf]);
+        }
+        if (!(ok = warp_wait(&red_full[buf], (it >> 1) & 1, abort_flag))) break;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) mt[h] = fmaxf(mt[h], rb[w * 12 + h]);
+          vref = fmaxf(vref, rb[w * 12 + kHeads]);
+        }
+        // P relative to the tile's maximum, V scales relative to the tile's largest
+        const float vrel = vref > 0.0f ? vs / vref : 0.0f;
+        float pr[kHeads], al[kHeads], be[kHeads];
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          const float mn = fmaxf(m[h], mt[h]);
+          al[h] = m[h] == -INFINITY ? 0.0f : ex2_approx(m[h] - mn);
+          be[h] = ex2_approx(mt[h] - mn);
+          m[h] = mn;
+          const float e = ex2_approx(s[h] - mt[h]);
+          l[h] = fmaf(e, be[h], l[h] * al[h]);
+          be[h] *= vref * (kInt8 ? 1.0f / kInt8One : 1.0f / 256.0f);
+          pr[h] = e * vrel;
+        }
+        uint8_t* pb = smem + Sm::p + buf * kCols * 128;
+        auto put = [&](int part, int h, uint32_t byte) {
+          const int n = part * kHeads + h;
+          pb[n * 128 + (((tid >> 4) ^ (n & 7)) << 4) + (tid & 15)] = static_cast<uint8_t>(byte);
+        };
+#pragma unroll
+        for (int h = 0; h < kHeads; h += 2) {
+          if constexpr (kInt8) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint32_t v = split_int8(pr[h + e]);
+#pragma unroll
+              for (int pt = 0; pt < kParts; ++pt) put(pt, h + e, v >> (16 - 8 * pt));
+            }
+          } else {
+            uint16_t part[kParts];
+            split_e4m3(__floats2half2_rn(pr[h] * 256.0f, pr[h + 1] * 256.0f), part);
+#pragma unroll
+            for (int pt = 0; pt < kParts; ++pt) {
+              put(pt, h, part[pt] & 0xFFu);
+              put(pt, h + 1, part[pt] >> 8);
+            }
+          }
+        }
+        if (key0 + kTile > seg.hi) {
+          // rows past the legal keys: whatever the cache holds there (a NaN byte, say) must not
+          // meet P = 0 in the product
+          const int st = it % kStages;
+          if (!(ok = warp_wait(&v_full[st], (it / kStages) & 1, abort_flag))) break;
+          if (!legal) {
+            uint4* row = reinterpret_cast<uint4*>(smem + Sm::v + st * kTileBytes + tid * 128);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
+          }
+        }
+        fence_proxy_async_smem();
+        tc_fence_before();
+        mbar_arrive(&p_full[buf]);
+        if (i > 0 && !(ok = take_o(it - 1))) break;
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h) {
+          alpha[h] = al[h];
+          beta[h] = be[h];
+        }
+      }
+      if (ok) ok = take_o(it - 1);
+      if (!ok) break;
+      // row sums over the keys (threads)
+      float* lb = lred + (nseg & 1) * 32;
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+#pragma unroll
+        for (int x = 1; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
+        if (lane == 0) lb[warp * 8 + h] = l[h];
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(l_full);
+      if (!(ok = warp_wait(l_full, nseg & 1, abort_flag))) break;
+      const int64_t slot = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + cta;
+#pragma unroll
+      for (int h = 0; h < kHeads; ++h) {
+        const float sum = (lb[h] + lb[8 + h]) + (lb[16 + h] + lb[24 + h]);
+        if (tid == h) reinterpret_cast<float2*>(p.part_ml)[slot * kHeads + h] = make_float2(m[h], sum);
+        if (h >= nh) continue;
+        if (seg.n == seg.all) {  // the whole unit: no merge
+          const int64_t row = static_cast<int64_t>(seg.cur_b) * p.Hq + head0 + h;
+          p.out[row * 128 + tid] = __float2bfloat16_rn(o[h] / sum);
+          if (tid == h) p.lse[row] = lg2_approx(sum) + m[h];
+        } else {
+          p.part_o[(slot * kHeads + h) * 128 + tid] = o[h];
+        }
+      }
+      ++nseg;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 5) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 4 * kCols);
+  }
+  if (tid == 0) p.cta_status[cta] = *abort_flag ? kStatusTimeout : 0;
+}
+
+// Second kernel.  Blocks [0, B Hq): one query head each, the merge of its unit's
+// segments (nothing where one CTA did the whole unit).  Blocks from there on (with
+// weights): an equal share of the (sequence, KV head, tile) items each, the weights
+// 2^(s - lse) of a tile's keys summed over the group's heads in a fixed order and
+// added to the accumulated ones.
+constexpr int kMaxCtas = 1024;
+
+struct UnitSplit {
+  int first, last;  // CTAs that worked on the unit
+};
+__device__ __forceinline__ UnitSplit unit_split(const KvDecodeParams& p, int b, int u, int n) {
+  const int units = p.Hkv * p.nhb;
+  const int tiles = p.cum[p.B] * units;
+  const int per = (tiles + p.ctas - 1) / p.ctas;
+  const int t0 = p.cum[b] * units + u * n;
+  return UnitSplit{t0 / per, (t0 + n - 1) / per};
+}
+
+__global__ void __launch_bounds__(128) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
+  __shared__ float wsh[kMaxCtas];
+  __shared__ float red[8];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int units = p.Hkv * p.nhb;
+  if (blockIdx.x == 0) {
+    int st = 0;
+    for (int c = tid; c < p.ctas; c += 128) st |= p.cta_status[c];
+    st = __syncthreads_or(st);
+    if (tid == 0) *p.status = st != 0 ? kStatusTimeout : 0;
+  }
+  const int n_heads = p.B * p.Hq;
+  if (static_cast<int>(blockIdx.x) < n_heads) {
+    const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq;
+    const int hr = hq % p.r;
+    const int u = (hq / p.r) * p.nhb + hr / p.heads, h = hr % p.heads;
+    const int n = p.cum[b + 1] - p.cum[b];
+    const int64_t row = blockIdx.x;
+    if (n == 0) {  // no key: 0 / 0 and log2 0, as the prefill writes a row without a legal key
+      p.out[row * 128 + tid] = __float2bfloat16_rn(__uint_as_float(0x7FC00000u));
+      if (tid == 0) p.lse[row] = -INFINITY;
+      return;
+    }
+    const UnitSplit us = unit_split(p, b, u, n);
+    if (us.first == us.last) return;
+    const int nseg = us.last - us.first + 1;
+    const int64_t slot0 = static_cast<int64_t>(b) * units + u + us.first;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * p.heads + h;
+    float M = -INFINITY;
+    for (int i = tid; i < nseg; i += 128) M = fmaxf(M, ml[static_cast<int64_t>(i) * p.heads].x);
+    M = warp_max(M);
+    if (lane == 0) red[warp] = M;
+    __syncthreads();
+    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+    float L = 0.0f;
+    for (int i = tid; i < nseg; i += 128) {
+      const float2 x = ml[static_cast<int64_t>(i) * p.heads];
+      const float w = ex2_approx(x.x - M);
+      wsh[i] = w;
+      L = fmaf(x.y, w, L);
+    }
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+    if (lane == 0) red[4 + warp] = L;
+    __syncthreads();
+    L = (red[4] + red[5]) + (red[6] + red[7]);
+    const float* po = p.part_o + (slot0 * p.heads + h) * 128 + tid;
+    float acc = 0.0f;
+#pragma unroll 8
+    for (int i = 0; i < nseg; ++i) acc = fmaf(po[static_cast<int64_t>(i) * p.heads * 128], wsh[i], acc);
+    p.out[row * 128 + tid] = __float2bfloat16_rn(acc / L);
+    if (tid == 0) p.lse[row] = lg2_approx(L) + M;
+    return;
+  }
+  // accumulated weights
+  const int share = gridDim.x - n_heads, me = blockIdx.x - n_heads;
+  const int items = p.cum[p.B] * p.Hkv;
+  const int per = (items + share - 1) / share;
+  int t = me * per;
+  const int t1 = min(items, t + per);
+  if (t >= t1) return;
+  int b = 0, last = p.B;  // cum[b] Hkv <= t < cum[b + 1] Hkv
+  while (last - b > 1) {
+    const int mid = (b + last) / 2;
+    if (p.cum[mid] * p.Hkv <= t) b = mid; else last = mid;
+  }
+  while (t < t1) {
+    while (p.cum[b + 1] * p.Hkv <= t) ++b;
+    const int n = p.cum[b + 1] - p.cum[b];
+    const int g = (t - p.cum[b] * p.Hkv) / n;
+    const int i0 = t - p.cum[b] * p.Hkv - g * n;
+    const int cnt = min(n - i0, t1 - t);
+    const KeyRange kr = key_range(p, b);
+    float* dst = p.weights + (static_cast<int64_t>(b) * p.Hkv + g) * p.Smax;
+    for (int hb = 0; hb < p.nhb; ++hb) {
+      const int u = g * p.nhb + hb;
+      const int nh = min(p.heads, p.r - hb * p.heads);
+      const UnitSplit us = unit_split(p, b, u, n);
+      const int nseg = us.last - us.first + 1;
+      const int64_t slot0 = static_cast<int64_t>(b) * units + u + us.first;
+      __syncthreads();
+      for (int h = warp; h < nh; h += 4) {  // lse of each head from its segments
+        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * p.heads + h;
+        float M = -INFINITY, L = 0.0f;
+        for (int i = lane; i < nseg; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * p.heads].x);
+        M = warp_max(M);
+        for (int i = lane; i < nseg; i += 32) {
+          const float2 x = ml[static_cast<int64_t>(i) * p.heads];
+          L = fmaf(x.y, ex2_approx(x.x - M), L);
+        }
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+        if (lane == 0) red[h] = lg2_approx(L) + M;
+      }
+      __syncthreads();
+      const float* sc = p.scores + (static_cast<int64_t>(p.cum[b]) * units + static_cast<int64_t>(u) * n + i0) * p.heads * kTile + tid;
+      for (int i = 0; i < cnt; ++i) {
+        const int key = kr.lo + (i0 + i) * kTile + tid;
+        float w = 0.0f;
+        for (int h = 0; h < nh; ++h) w += ex2_approx(sc[(static_cast<int64_t>(i) * p.heads + h) * kTile] - red[h]);
+        if (key < kr.hi) dst[key] += w;
+      }
+    }
+    t += cnt;
+  }
+}
+
+template <bool kInt8, int kHeads, bool kWeights>
+cudaError_t launch_main(const KvDecodeParams& p, cudaStream_t stream) {
+  static bool attr_set[64] = {};
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  if (dev >= 64 || !attr_set[dev]) {
+    e = cudaFuncSetAttribute(kv_decode_kernel<kInt8, kHeads, kWeights>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             KvSmem<kHeads>::bytes);
+    if (e != cudaSuccess) return e;
+    if (dev < 64) attr_set[dev] = true;
+  }
+  kv_decode_kernel<kInt8, kHeads, kWeights><<<p.ctas, kThreads, KvSmem<kHeads>::bytes, stream>>>(p);
+  return cudaGetLastError();
+}
+
+template <bool kInt8>
+cudaError_t launch_for(const KvDecodeParams& p, cudaStream_t stream) {
+  const bool w = p.weights != nullptr;
+  if (p.heads == 4) return w ? launch_main<kInt8, 4, true>(p, stream) : launch_main<kInt8, 4, false>(p, stream);
+  return w ? launch_main<kInt8, 8, true>(p, stream) : launch_main<kInt8, 8, false>(p, stream);
+}
+
+}  // namespace
+
+cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream) {
+  cudaError_t e = int8 ? launch_for<true>(p, stream) : launch_for<false>(p, stream);
+  if (e != cudaSuccess) return e;
+  const int extra = p.weights != nullptr ? p.ctas : 0;
+  kv_decode_merge_kernel<<<p.B * p.Hq + extra, 128, 0, stream>>>(p);
+  return cudaGetLastError();
+}
+
+}  // namespace swa

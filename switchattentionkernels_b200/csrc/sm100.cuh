@@ -103,6 +103,15 @@ __device__ __forceinline__ void tma_load_2d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
+                                            int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2)
+      : "memory");
+}
+
 __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1,
                                             int c2, int c3) {
   asm volatile(
@@ -302,6 +311,34 @@ __device__ __forceinline__ void umma_ts_k128_bhalf8k_warp(uint32_t d_tmem, uint3
       : "memory");
 }
 
+// Four back-to-back SS MMAs over K = 128 of 8-bit operands (K = 32 each), kind::f8f6f4
+// with e4m3 operands and FP32 accumulation, or kind::i8 with signed bytes and INT32
+// accumulation; step k adds k * a_step / k * b_step (descriptor units of 16 bytes) to
+// the operands' start addresses.  The first step overwrites D.
+template <bool kInt8>
+__device__ __forceinline__ void umma8_ss_k128_warp(uint32_t d_tmem, uint64_t a, uint64_t b, uint32_t a_step,
+                                                   uint32_t b_step, uint32_t idesc) {
+  const uint64_t a1 = a + a_step, a2 = a + 2 * a_step, a3 = a + 3 * a_step;
+  const uint64_t b1 = b + b_step, b2 = b + 2 * b_step, b3 = b + 3 * b_step;
+#define SWA_UMMA8(kind)                                                           \
+  asm volatile(                                                                   \
+      "{\n\t.reg .pred e, p0, p1;\n\t"                                            \
+      "setp.ne.b32 p0, 0, 0;\n\tsetp.eq.b32 p1, 0, 0;\n\t"                        \
+      "elect.sync _|e, 0xffffffff;\n\t"                                          \
+      "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], %1, %5, %9, p0;\n\t"     \
+      "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], %2, %6, %9, p1;\n\t"     \
+      "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], %3, %7, %9, p1;\n\t"     \
+      "@e tcgen05.mma.cta_group::1.kind::" kind " [%0], %4, %8, %9, p1;\n\t}" :: \
+          "r"(d_tmem), "l"(a), "l"(a1), "l"(a2), "l"(a3), "l"(b), "l"(b1), "l"(b2), "l"(b3), "r"(idesc) \
+      : "memory")
+  if constexpr (kInt8) {
+    SWA_UMMA8("i8");
+  } else {
+    SWA_UMMA8("f8f6f4");
+  }
+#undef SWA_UMMA8
+}
+
 // Shared-memory matrix descriptor, 128-byte swizzle, sm100 version field = 1.
 //   K-major operand : lbo ignored (pass 16), sbo = byte stride between 8-row groups.
 //   MN-major operand: lbo = byte stride between 64-element MN blocks,
@@ -321,6 +358,18 @@ __host__ __device__ constexpr uint32_t make_idesc_bf16_f32(int M, int N, bool a_
   return (1u << 4)                                   // D format: F32
          | (1u << 7)                                 // A format: BF16
          | (1u << 10)                                // B format: BF16
+         | ((a_mn_major ? 1u : 0u) << 15)            // A major
+         | ((b_mn_major ? 1u : 0u) << 16)            // B major
+         | (static_cast<uint32_t>(N >> 3) << 17)     // N / 8
+         | (static_cast<uint32_t>(M >> 4) << 24);    // M / 16
+}
+
+// Instruction descriptor for 8-bit operands: kind::f8f6f4 with e4m3 A/B and FP32 D, or
+// kind::i8 with signed A/B and INT32 D.
+__host__ __device__ constexpr uint32_t make_idesc_8bit(bool int8, int M, int N, bool a_mn_major, bool b_mn_major) {
+  return (int8 ? 2u : 1u) << 4                       // D format: S32 / F32
+         | (int8 ? 1u : 0u) << 7                     // A format: signed 8-bit / e4m3
+         | (int8 ? 1u : 0u) << 10                    // B format
          | ((a_mn_major ? 1u : 0u) << 15)            // A major
          | ((b_mn_major ? 1u : 0u) << 16)            // B major
          | (static_cast<uint32_t>(N >> 3) << 17)     // N / 8

@@ -1,0 +1,285 @@
+"""Block-scaled 8-bit KV cache: append, decode attention, eviction.
+
+Not part of the reference (its kernels are prefill only).  ``switch_gqa_decode_forward``
+reads an e4m3 cache with one scale per (sequence, KV head), which has to be known
+before the first token is cached; here every block of 16 to 128 rows of a KV head has
+its own scale, made as the rows arrive.  The three operators of a serving loop:
+
+* ``switch_kv_cache_append``: BF16 K/V rows (a prompt, a chunk, one token) into the cache;
+* ``switch_gqa_decode_cached``: the decode step over it, routed full or window per
+  sequence as ``switch_gqa_decode_forward`` is, which can also accumulate the attention
+  weight that every cached key received;
+* ``switch_kv_cache_evict``: cuts every sequence to a budget of rows, keeping the first
+  and last ones and, of the rest, those with the largest accumulated weight.
+
+All three run on the current stream of the cache's device, read lengths on the device,
+never synchronise and can be captured into a CUDA graph.
+"""
+from __future__ import annotations
+
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from . import _core, _native
+from ._core import LOG2E
+
+HEAD_DIM = 128
+BLOCK_SIZES = (16, 32, 64, 128)
+_DTYPES = {torch.float8_e4m3fn: _native.KV_E4M3, torch.int8: _native.KV_INT8}
+
+
+@dataclass
+class SwitchKVCache:
+    """A batch's cache.  The rows of one KV head lie together; value = byte * scale.
+
+    Row ``s`` of (sequence ``b``, KV head ``g``) belongs to block ``s // block_size`` of it.
+    Rows from ``seq_lens[b]`` on hold nothing.  Scales are FP32 and non-negative
+    (``switch_kv_cache_append`` makes powers of two; the other operators take any).
+    """
+    k: torch.Tensor                           # float8_e4m3fn or int8 [B, Hkv, Smax, 128]
+    v: torch.Tensor
+    k_scale: torch.Tensor                     # float32 [B, Hkv, ceil(Smax / block_size)]
+    v_scale: torch.Tensor
+    seq_lens: torch.Tensor                    # int32 [B] cached rows of each sequence
+    key_weights: torch.Tensor | None = None   # float32 [B, Hkv, Smax] accumulated attention weight
+    block_size: int = 64
+
+
+def make_switch_kv_cache(batch: int, max_len: int, kv_heads: int, *, device, dtype: torch.dtype = torch.float8_e4m3fn,
+                         block_size: int = 64, track_weights: bool = False) -> SwitchKVCache:
+    """An empty cache of ``max_len`` rows per sequence; ``track_weights`` adds ``key_weights``."""
+    if batch <= 0 or max_len <= 0 or kv_heads <= 0:
+        raise ValueError("batch, max_len and kv_heads must be positive")
+    if dtype not in _DTYPES:
+        raise TypeError("dtype must be float8_e4m3fn or int8")
+    if block_size not in BLOCK_SIZES:
+        raise ValueError("block_size must be 16, 32, 64 or 128")
+    blocks = -(-max_len // block_size)
+    rows = lambda: torch.zeros((batch, kv_heads, max_len, HEAD_DIM), dtype=torch.int8, device=device).view(dtype)  # noqa: E731
+    scales = lambda: torch.zeros((batch, kv_heads, blocks), dtype=torch.float32, device=device)  # noqa: E731
+    weights = torch.zeros((batch, kv_heads, max_len), dtype=torch.float32, device=device) if track_weights else None
+    return SwitchKVCache(rows(), rows(), scales(), scales(), torch.zeros(batch, dtype=torch.int32, device=device),
+                         weights, block_size)
+
+
+def _check_cache(cache: SwitchKVCache, name: str = "cache") -> tuple[int, int, int]:
+    """``(B, Hkv, Smax)`` of a well-formed cache."""
+    if not isinstance(cache, SwitchKVCache):
+        raise TypeError(f"{name} must be a SwitchKVCache")
+    k, v = cache.k, cache.v
+    if not isinstance(k, torch.Tensor) or k.dtype not in _DTYPES or not k.is_cuda:
+        raise TypeError(f"{name}.k must be a device-resident float8_e4m3fn or int8 tensor")
+    if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or not v.is_cuda:
+        raise TypeError(f"{name}.v must be a device-resident tensor of {name}.k's dtype")
+    if k.ndim != 4 or v.shape != k.shape:
+        raise ValueError(f"{name}.k and {name}.v must be [B, Hkv, Smax, 128]")
+    B, Hkv, Smax, D = k.shape
+    if D != HEAD_DIM:
+        raise ValueError("head_dim must be 128")
+    if B == 0 or Hkv == 0 or Smax == 0:
+        raise ValueError(f"{name} is empty")
+    if cache.block_size not in BLOCK_SIZES:
+        raise ValueError("block_size must be 16, 32, 64 or 128")
+    blocks = -(-Smax // cache.block_size)
+    expected = [("v", v, k.dtype, (B, Hkv, Smax, D)), ("k", k, k.dtype, (B, Hkv, Smax, D)),
+                ("k_scale", cache.k_scale, torch.float32, (B, Hkv, blocks)),
+                ("v_scale", cache.v_scale, torch.float32, (B, Hkv, blocks)),
+                ("seq_lens", cache.seq_lens, torch.int32, (B,))]
+    if cache.key_weights is not None:
+        expected.append(("key_weights", cache.key_weights, torch.float32, (B, Hkv, Smax)))
+    for field, t, dtype, shape in expected:
+        if (not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape or t.device != k.device
+                or not t.is_contiguous()):
+            raise ValueError(f"{name}.{field} must be a contiguous {dtype} {list(shape)} tensor on the device of {name}.k")
+    return B, Hkv, Smax
+
+
+def _check_rows(t, name: str, shape: tuple, dev) -> None:
+    if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda:
+        raise TypeError(f"{name} must be a device-resident bfloat16 tensor")
+    if t.device != dev:
+        raise ValueError(f"{name} must be on the device of the cache")
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}")
+    # a slice of a fused projection is fine: only the 128 values of a row have to lie together
+    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+        raise ValueError(f"{name} needs contiguous, 16-byte aligned rows (other strides multiples of 8 elements)")
+
+
+def _check_lens(t, name: str, B: int, dev) -> None:
+    if (not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32 or tuple(t.shape) != (B,)
+            or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 [B] tensor on the device of the cache")
+
+
+def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: torch.Tensor, *,
+                           new_lens: torch.Tensor | None = None, start: torch.Tensor | None = None) -> None:
+    """Write new K/V rows behind each sequence's cached ones; ``cache.seq_lens`` is advanced.
+
+    ``k_new`` / ``v_new``: BF16 ``[B, T, Hkv, 128]``, or ``[B, Hkv, 128]`` for one token per
+    sequence; views with contiguous rows (slices of a fused projection) are taken as
+    they are.  ``new_lens``: int32 ``[B]``, the rows of a padded batch that count (default:
+    all ``T``).  ``start``: int32 ``[B]``, the row at which each sequence's new rows begin
+    (default ``cache.seq_lens``; earlier: the rows from there on are replaced, e.g. after
+    rejected draft tokens).  Rows that do not fit (``>= Smax``) are dropped.
+
+    A block's scale is the smallest power of two that its rows need, and only grows:
+    when it does, the block's earlier rows are rounded again.  Rounding is to nearest
+    even; infinities saturate and do not count for the scale, NaN stays NaN in an e4m3
+    cache and becomes 0 in an int8 one.  Appended rows start with ``key_weights`` 0.
+    """
+    B, Hkv, Smax = _check_cache(cache)
+    dev = cache.k.device
+    token = isinstance(k_new, torch.Tensor) and k_new.ndim == 3
+    if not isinstance(k_new, torch.Tensor) or k_new.ndim not in (3, 4):
+        raise ValueError("k_new must have shape [B, T, Hkv, 128] or [B, Hkv, 128]")
+    T = 1 if token else int(k_new.shape[1])
+    shape = (B, Hkv, HEAD_DIM) if token else (B, T, Hkv, HEAD_DIM)
+    _check_rows(k_new, "k_new", shape, dev)
+    _check_rows(v_new, "v_new", shape, dev)
+    if new_lens is not None:
+        _check_lens(new_lens, "new_lens", B, dev)
+    if start is None:
+        start = cache.seq_lens
+    else:
+        _check_lens(start, "start", B, dev)
+    if T == 0:
+        return
+    strides = []
+    for t in (k_new, v_new):
+        st = t.stride()
+        strides.append((ctypes.c_int64 * 3)(st[0], 0 if token else st[1], st[1] if token else st[2]))
+    lib = _native.load()
+    with torch.cuda.device(dev):
+        rc = lib.swa_kv_append(_native.ptr(k_new), _native.ptr(v_new), strides[0], strides[1], _native.ptr(start),
+                               _native.ptr(new_lens), _native.ptr(cache.k), _native.ptr(cache.v),
+                               _native.ptr(cache.k_scale), _native.ptr(cache.v_scale),
+                               _native.ptr(cache.key_weights), _native.ptr(cache.seq_lens), B, T, Hkv, Smax, HEAD_DIM,
+                               cache.block_size, _DTYPES[cache.k.dtype], _native.stream_ptr(dev))
+    _native.check(rc, "switch_kv_cache_append")
+
+
+def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: torch.Tensor, *,
+                             window_size: int = 1024, sm_scale: float | None = None, accumulate: bool = True,
+                             status_out: torch.Tensor | None = None):
+    """Attention of each sequence's new token over its cached rows (the new one's included).
+
+    ``q``: BF16 ``[B, Hq, 128]`` or ``[B, 1, Hq, 128]`` (views with contiguous rows are
+    taken as they are), ``Hq`` a multiple of the cache's KV heads; ``route_full``: bool
+    ``[B]``, True = all cached rows, False = the last ``window_size`` of them.  Returns
+    ``(O, LSE)``: BF16 ``[B, Hq, 128]`` and FP32 ``[B, Hq]`` (log2 units), shaped like ``q``;
+    a sequence without rows gets O = NaN, LSE = -inf.  A query with an infinity or NaN
+    gets NaN in both.
+
+    With ``accumulate`` and a cache that has ``key_weights``, the softmax weight of every
+    row that was attended to, summed over the query heads of its KV head, is added to
+    them.  ``status_out``: as in ``switch_gqa_decode_forward``.
+    """
+    B, Hkv, Smax = _check_cache(cache)
+    dev = cache.k.device
+    squeeze = isinstance(q, torch.Tensor) and q.ndim == 4
+    if squeeze:
+        if q.shape[1] != 1:
+            raise ValueError("decode takes one query token per sequence")
+        q = q[:, 0]
+    if not isinstance(q, torch.Tensor) or q.ndim != 3:
+        raise ValueError("q must have shape [B, Hq, 128] or [B, 1, Hq, 128]")
+    Hq = int(q.shape[1])
+    _check_rows(q, "q", (B, Hq, HEAD_DIM), dev)
+    if Hq == 0 or Hq % Hkv != 0:
+        raise ValueError("query heads must be divisible by KV heads")
+    if window_size <= 0:
+        raise ValueError("window_size must be positive")
+    if (not isinstance(route_full, torch.Tensor) or route_full.device != dev or route_full.dtype != torch.bool
+            or tuple(route_full.shape) != (B,)):
+        raise ValueError("route_full must be a bool [B] tensor on the device of the cache")
+    scale = (sm_scale if sm_scale is not None else (1.0 / HEAD_DIM) ** 0.5) * LOG2E
+    if not scale > 0:
+        raise ValueError("sm_scale must be positive")
+    _core._check_status_out(status_out, dev)
+    weights = cache.key_weights if accumulate else None
+    lib = _native.load()
+    out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
+    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    with torch.cuda.device(dev):
+        nbytes = int(lib.swa_kv_decode_workspace_bytes(B, Smax, Hq, Hkv, int(weights is not None)))
+        if nbytes <= 0:
+            raise RuntimeError("decode workspace size query failed: " +
+                               lib.swa_last_error_string().decode(errors="replace"))
+        ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.int32, device=dev)
+        route = route_full.contiguous().view(torch.uint8)
+        rc = lib.swa_kv_decode(_native.ptr(q), q.stride(0), q.stride(1), _native.ptr(cache.k), _native.ptr(cache.v),
+                               _native.ptr(cache.k_scale), _native.ptr(cache.v_scale), _native.ptr(cache.seq_lens),
+                               _native.ptr(route), _native.ptr(out), _native.ptr(lse), _native.ptr(weights), B, Smax,
+                               Hq, Hkv, HEAD_DIM, cache.block_size, min(int(window_size), Smax), float(scale),
+                               _DTYPES[cache.k.dtype], _native.ptr(ws), ws.numel() * 4, _native.stream_ptr(dev))
+    _native.check(rc, "switch_gqa_decode_cached")
+    if status_out is not None or _core.CHECK_DEVICE_STATUS:
+        _core.publish_status(ws[0:1], status_out)
+    if squeeze:
+        return out.unsqueeze(1), lse.unsqueeze(1)
+    return out, lse
+
+
+def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, recent: int = 0,
+                          out: SwitchKVCache | None = None) -> torch.Tensor:
+    """Cut every sequence longer than ``keep`` rows to ``keep`` of them; needs ``key_weights``.
+
+    Each KV head keeps its first ``sink`` rows, its last ``recent`` rows and, of those
+    between, the ones with the largest ``key_weights`` (ties: the lowest row; NaN: last),
+    moved together in their order with their weights.  Shorter sequences keep all rows.
+    A sequence's sliding window keeps its meaning while ``recent >= window_size``: window
+    rows are the last cached ones.  A block's new scale is the largest of its rows'
+    scales; rows of a smaller one are rounded again.
+
+    In place by default.  ``out``: another cache of the same batch, heads, dtype and block
+    size, sharing no memory with ``cache`` and with at least ``min(keep, Smax)`` rows,
+    that takes the result; ``cache`` is then left as it is.  Returns int32
+    ``[B, Hkv, min(keep, Smax)]``: the former row of each kept row, -1 past the last one.
+    """
+    B, Hkv, Smax = _check_cache(cache)
+    dev = cache.k.device
+    if cache.key_weights is None:
+        raise ValueError("eviction needs a cache with key_weights")
+    keep, sink, recent = int(keep), int(sink), int(recent)
+    if keep <= 0 or sink < 0 or recent < 0 or sink + recent > keep:
+        raise ValueError("keep must be positive and at least sink + recent, both non-negative")
+    if keep >= Smax:  # no sequence is longer
+        keep, sink, recent = Smax, 0, 0
+    n = keep
+    dst = cache
+    if out is not None and out is not cache:
+        Bo, Ho, So = _check_cache(out, "out")
+        if (Bo, Ho) != (B, Hkv) or out.k.dtype != cache.k.dtype or out.block_size != cache.block_size:
+            raise ValueError("out must have the batch, heads, dtype and block size of the cache")
+        if out.k.device != dev:
+            raise ValueError("out must be on the device of the cache")
+        if out.key_weights is None:
+            raise ValueError("out must have key_weights")
+        if So < n:
+            raise ValueError("out holds fewer rows than are kept")
+        mine = [_extent(t) for t in _tensors(cache)]
+        if any(a0 < b1 and b0 < a1 for a0, a1 in (_extent(t) for t in _tensors(out)) for b0, b1 in mine):
+            raise ValueError("out must not share memory with the cache")
+        dst = out
+    slots = torch.empty((B, Hkv, n), dtype=torch.int32, device=dev)
+    lib = _native.load()
+    with torch.cuda.device(dev):
+        rc = lib.swa_kv_evict(_native.ptr(cache.k), _native.ptr(cache.v), _native.ptr(cache.k_scale),
+                              _native.ptr(cache.v_scale), _native.ptr(cache.key_weights), _native.ptr(cache.seq_lens),
+                              _native.ptr(dst.k), _native.ptr(dst.v), _native.ptr(dst.k_scale),
+                              _native.ptr(dst.v_scale), _native.ptr(dst.key_weights), _native.ptr(dst.seq_lens),
+                              _native.ptr(slots), B, Hkv, Smax, int(dst.k.shape[2]), HEAD_DIM, cache.block_size, keep,
+                              sink, recent, _DTYPES[cache.k.dtype], _native.stream_ptr(dev))
+    _native.check(rc, "switch_kv_cache_evict")
+    return slots
+
+
+def _tensors(cache: SwitchKVCache):
+    return (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.seq_lens, cache.key_weights)
+
+
+def _extent(t: torch.Tensor) -> tuple[int, int]:
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
