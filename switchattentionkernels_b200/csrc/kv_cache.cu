@@ -238,15 +238,17 @@ cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
 // ---------------------------------------------------------------------------
 // evict: selection
 // ---------------------------------------------------------------------------
-// One cluster of 8 CTAs per (sequence, KV head), each CTA a contiguous eighth of the
+// A cluster of 1 to 8 CTAs per (sequence, KV head), each CTA a contiguous part of the
 // rows and each warp a contiguous part of that.  The k-th largest weight of the
 // rows between the sink and the recent ones comes from a radix selection (digits
 // of 11, 11 and 10 bits of the order-preserving integer form; the CTAs' histograms
-// are added up through distributed shared memory), then a counting pass and an
-// emitting pass write the kept rows in order, rows equal to the threshold from the
-// lowest index on.  The weights are read five times, all but the first from L2.
-constexpr int kSelThreads = 512;
-constexpr int kSelCluster = 8;
+// are added up through distributed shared memory), then the kept rows of each warp are
+// counted and written in order, rows equal to the threshold from the lowest index on.
+// Latency-bound (a chain of a dozen barriers over little data), so the weights are
+// read once and stay in registers, kPerThread of them a thread; with kPerThread = 0
+// (more rows than 8 CTAs can hold) every pass reads them again, from L2.
+constexpr int kSelThreads = 1024;
+constexpr int kSelMaxCluster = 8;
 constexpr int kSelBins = 2048;
 constexpr int kSelWarps = kSelThreads / 32;
 
@@ -257,30 +259,51 @@ __device__ __forceinline__ uint32_t order_bits(float w) {
   return u ^ ((u >> 31) != 0u ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-__global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThreads)
-    kv_select_kernel(const __grid_constant__ KvEvictParams p) {
+template <int kPerThread>
+__global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ KvEvictParams p) {
   __shared__ uint32_t hist[3][kSelBins];
   __shared__ uint32_t warp_sum[kSelWarps];
   __shared__ uint32_t found[2];
   __shared__ uint32_t warp_gt[kSelWarps], warp_eq[kSelWarps];
   __shared__ uint32_t cta_cnt[2];
   cg::cluster_group cluster = cg::this_cluster();
-  const int64_t unit = blockIdx.x / kSelCluster;
-  const int rank = blockIdx.x % kSelCluster;
+  const int ncta = static_cast<int>(cluster.num_blocks());
+  const int rank = static_cast<int>(cluster.block_rank());
+  const int64_t unit = blockIdx.x / ncta;
   const int b = static_cast<int>(unit / p.Hkv);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int L = min(max(p.seq_lens[b], 0), p.Smax);
   int32_t* slots = p.slots + unit * p.n;
   if (L <= p.keep) {  // nothing to evict (the whole cluster agrees)
-    for (int i = rank * kSelThreads + tid; i < p.n; i += kSelCluster * kSelThreads) slots[i] = i < L ? i : -1;
+    for (int i = rank * kSelThreads + tid; i < p.n; i += ncta * kSelThreads) slots[i] = i < L ? i : -1;
     return;
   }
   const float* w = p.src_weights + unit * p.Smax;
-  const int per_warp = ((L + kSelCluster * kSelWarps - 1) / (kSelCluster * kSelWarps) + 31) & ~31;
-  const int cta0 = rank * per_warp * kSelWarps;
-  const int cta1 = min(L, cta0 + per_warp * kSelWarps);
+  const int all_warps = ncta * kSelWarps;
+  const int per_warp = ((L + all_warps - 1) / all_warps + 31) & ~31;
+  const int w0 = min(L, (rank * kSelWarps + warp) * per_warp), w1 = min(L, w0 + per_warp);
   const int lo = p.sink, hi = L - p.recent;  // candidates (L > keep >= sink + recent)
-  const int c0 = max(cta0, lo), c1 = min(cta1, hi);
+  uint32_t key[kPerThread > 0 ? kPerThread : 1];
+  if constexpr (kPerThread > 0) {
+    float x[kPerThread];
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) {
+      const int i = w0 + 32 * j + lane;
+      x[j] = i < w1 ? w[i] : 0.0f;
+    }
+#pragma unroll
+    for (int j = 0; j < kPerThread; ++j) key[j] = order_bits(x[j]);
+  }
+  // calls f(row, key of the row if it is one of the warp's) for the warp's rows, 32 at a time
+  auto each = [&](auto&& f) {
+    if constexpr (kPerThread > 0) {
+#pragma unroll
+      for (int j = 0; j < kPerThread; ++j)
+        if (w0 + 32 * j < w1) f(w0 + 32 * j + lane, key[j]);
+    } else {
+      for (int i0 = w0; i0 < w1; i0 += 32) f(i0 + lane, i0 + lane < w1 ? order_bits(w[i0 + lane]) : 0u);
+    }
+  };
   uint32_t need = static_cast<uint32_t>(p.keep - p.sink - p.recent);  // < hi - lo
   uint32_t thr = 0xFFFFFFFFu;  // need == 0: no weight is above it, and no equal one is taken
   if (need > 0) {
@@ -291,23 +314,19 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
     for (int pass = 0; pass < 3; ++pass) {
       const int shift = pass == 0 ? 21 : (pass == 1 ? 10 : 0);
       const uint32_t dmask = pass == 2 ? 1023u : 2047u;
-      const int up = pass == 0 ? 0 : (pass == 1 ? 21 : 10);  // the digits above: u >> up == pfx
-      for (int i = c0 + tid; i < c1; i += kSelThreads) {
-        const uint32_t u = order_bits(w[i]);
-        if (pass == 0 || (u >> up) == pfx) atomicAdd(&hist[pass][(u >> shift) & dmask], 1u);
-      }
+      const int up = pass == 1 ? 21 : 10;  // the digits above: u >> up == pfx
+      each([&](int i, uint32_t u) {
+        if (i < w1 && i >= lo && i < hi && (pass == 0 || (u >> up) == pfx)) atomicAdd(&hist[pass][(u >> shift) & dmask], 1u);
+      });
       cluster.sync();
-      // bins 4 tid .. 4 tid + 3 over the whole cluster, then the sum of the bins above them
-      uint4 mine = make_uint4(0, 0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < kSelCluster; ++r) {
-        const uint4 h = reinterpret_cast<const uint4*>(cluster.map_shared_rank(&hist[pass][0], r))[tid];
+      // bins 2 tid and 2 tid + 1 over the whole cluster, then the sum of the bins above them
+      uint2 mine = make_uint2(0, 0);
+      for (int r = 0; r < ncta; ++r) {
+        const uint2 h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[pass][0], r))[tid];
         mine.x += h.x;
         mine.y += h.y;
-        mine.z += h.z;
-        mine.w += h.w;
       }
-      const uint32_t total = mine.x + mine.y + mine.z + mine.w;
+      const uint32_t total = mine.x + mine.y;
       uint32_t suffix = total;  // over this lane and the lanes above it
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -316,81 +335,88 @@ __global__ void __cluster_dims__(kSelCluster, 1, 1) __launch_bounds__(kSelThread
       }
       if (lane == 0) warp_sum[warp] = suffix;
       __syncthreads();
-      uint32_t above = suffix - total;
-      for (int k = warp + 1; k < kSelWarps; ++k) above += warp_sum[k];
+      uint32_t above = __reduce_add_sync(0xffffffffu, lane > warp ? warp_sum[lane] : 0u) + suffix - total;
       if (above < need && above + total >= need) {  // exactly one thread
-        const uint32_t bin[4] = {mine.x, mine.y, mine.z, mine.w};
-        int d = 3;
-        while (d > 0 && above + bin[d] < need) above += bin[d--];
-        found[0] = static_cast<uint32_t>(4 * tid + d);
+        const bool top = above + mine.y >= need;
+        if (!top) above += mine.y;
+        found[0] = static_cast<uint32_t>(2 * tid + (top ? 1 : 0));
         found[1] = need - above;
       }
       __syncthreads();
-      pfx = pass == 2 ? (pfx << 10) | found[0] : (pfx << 11) | found[0];
+      pfx = (pfx << (pass == 2 ? 10 : 11)) | found[0];
       need = found[1];
-      __syncthreads();
     }
     thr = pfx;
   }
-  // rows above the threshold (and the sink and recent rows) and rows equal to it, per warp
-  const int w0 = cta0 + warp * per_warp, w1 = min(cta1, w0 + per_warp);
-  auto classify = [&](int i, bool& gt, bool& eq) {
-    gt = eq = false;
-    if (i < w1) {
-      if (i < lo || i >= hi) {
-        gt = true;
-      } else {
-        const uint32_t u = order_bits(w[i]);
-        gt = u > thr;
-        eq = u == thr;
-      }
-    }
+  // rows above the threshold (and the sink and recent rows) and rows equal to it
+  auto classify = [&](int i, uint32_t u, uint32_t& gt, uint32_t& eq) {
+    const bool safe = i < lo || i >= hi;
+    gt = __ballot_sync(0xffffffffu, i < w1 && (safe || u > thr));
+    eq = __ballot_sync(0xffffffffu, i < w1 && !safe && u == thr);
   };
   uint32_t ngt = 0, neq = 0;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    bool gt, eq;
-    classify(i0 + lane, gt, eq);
-    ngt += __popc(__ballot_sync(0xffffffffu, gt));
-    neq += __popc(__ballot_sync(0xffffffffu, eq));
-  }
+  each([&](int i, uint32_t u) {
+    uint32_t gt, eq;
+    classify(i, u, gt, eq);
+    ngt += __popc(gt);
+    neq += __popc(eq);
+  });
   if (lane == 0) {
     warp_gt[warp] = ngt;
     warp_eq[warp] = neq;
   }
   __syncthreads();
-  uint32_t gt_before = 0, eq_before = 0, gt_all = 0, eq_all = 0;
-  for (int k = 0; k < kSelWarps; ++k) {
-    if (k < warp) {
-      gt_before += warp_gt[k];
-      eq_before += warp_eq[k];
+  uint32_t gt_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_gt[lane] : 0u);
+  uint32_t eq_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_eq[lane] : 0u);
+  if (ncta > 1) {
+    if (warp == kSelWarps - 1 && lane == 0) {
+      cta_cnt[0] = gt_before + ngt;
+      cta_cnt[1] = eq_before + neq;
     }
-    gt_all += warp_gt[k];
-    eq_all += warp_eq[k];
+    cluster.sync();
+    for (int r = 0; r < rank; ++r) {
+      const uint32_t* other = cluster.map_shared_rank(&cta_cnt[0], r);
+      gt_before += other[0];
+      eq_before += other[1];
+    }
+    cluster.sync();  // the counts (and histograms) of a CTA are read no more: it may exit
   }
-  if (tid == 0) {
-    cta_cnt[0] = gt_all;
-    cta_cnt[1] = eq_all;
-  }
-  cluster.sync();
-  for (int r = 0; r < rank; ++r) {
-    const uint32_t* other = cluster.map_shared_rank(&cta_cnt[0], r);
-    gt_before += other[0];
-    eq_before += other[1];
-  }
-  cluster.sync();  // the counts (and histograms) of a CTA are read no more: it may exit
   const uint32_t below = (1u << lane) - 1u;
-  for (int i0 = w0; i0 < w1; i0 += 32) {
-    bool gt, eq;
-    classify(i0 + lane, gt, eq);
-    const uint32_t bg = __ballot_sync(0xffffffffu, gt), be = __ballot_sync(0xffffffffu, eq);
-    const uint32_t er = eq_before + __popc(be & below);
-    if (gt || (eq && er < need)) {
-      const uint32_t at = gt_before + __popc(bg & below) + min(er, need);
-      slots[at] = i0 + lane;
-    }
-    gt_before += __popc(bg);
-    eq_before += __popc(be);
-  }
+  each([&](int i, uint32_t u) {
+    uint32_t gt, eq;
+    classify(i, u, gt, eq);
+    const uint32_t er = eq_before + __popc(eq & below);
+    if (((gt >> lane) & 1u) != 0u || (((eq >> lane) & 1u) != 0u && er < need))
+      slots[gt_before + __popc(gt & below) + min(er, need)] = i;
+    gt_before += __popc(gt);
+    eq_before += __popc(eq);
+  });
+}
+
+template <int kPerThread>
+cudaError_t launch_select(const KvEvictParams& p, int cluster, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(p.B * p.Hkv * cluster);
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cluster;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kv_select_kernel<kPerThread>, p);
+}
+
+// CTAs per (sequence, KV head): 8 weights a thread, as few CTAs as hold a sequence of
+// the largest length; above 8 CTAs' 65536 rows 16 a thread, above 131072 none are held.
+cudaError_t launch_select(const KvEvictParams& p, cudaStream_t stream) {
+  int cluster = 1;
+  while (cluster < kSelMaxCluster && p.Smax > cluster * kSelThreads * 8) cluster *= 2;
+  if (p.Smax <= cluster * kSelThreads * 8) return launch_select<8>(p, cluster, stream);
+  if (p.Smax <= cluster * kSelThreads * 16) return launch_select<16>(p, cluster, stream);
+  return launch_select<0>(p, cluster, stream);
 }
 
 // ---------------------------------------------------------------------------
@@ -538,8 +564,7 @@ cudaError_t launch_kv_append(const KvAppendParams& p, bool int8, cudaStream_t st
 
 cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream) {
   const int units = p.B * p.Hkv;
-  kv_select_kernel<<<units * kSelCluster, kSelThreads, 0, stream>>>(p);
-  cudaError_t e = cudaGetLastError();
+  cudaError_t e = launch_select(p, stream);
   if (e != cudaSuccess) return e;
   if (in_place) {
     if (int8) {
