@@ -81,12 +81,70 @@ __device__ __forceinline__ uint32_t finite_abs_max(uint32_t pair) {
   hi = hi < 0x7F80u ? hi : 0u;
   return max(lo, hi);
 }
-__device__ __forceinline__ uint32_t abs_max_bits(uint4 v) {
-  return max(max(finite_abs_max(v.x), finite_abs_max(v.y)), max(finite_abs_max(v.z), finite_abs_max(v.w)));
+
+// The same over N x 8 values, two at a time in packed 16-bit maxima; the values are
+// looked at one by one only where an infinity or NaN is among them (`finite` false).
+template <int N>
+__device__ __forceinline__ uint32_t abs_max_bits(const uint4* v, bool& finite) {
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m = __vmaxu2(m, v[i].x & 0x7FFF7FFFu);
+    m = __vmaxu2(m, v[i].y & 0x7FFF7FFFu);
+    m = __vmaxu2(m, v[i].z & 0x7FFF7FFFu);
+    m = __vmaxu2(m, v[i].w & 0x7FFF7FFFu);
+  }
+  m = max(m & 0xFFFFu, m >> 16);
+  finite = m < 0x7F80u;
+  if (!finite) {
+    m = 0u;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      m = max(max(m, max(finite_abs_max(v[i].x), finite_abs_max(v[i].y))), max(finite_abs_max(v[i].z), finite_abs_max(v[i].w)));
+  }
+  return m;
 }
 
 __device__ __forceinline__ float bf_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
+
+// Eight BF16 values times `inv` (a power of two that brings finite ones within 127 /
+// 448) to 8 bits.  The append is bound by instructions before it is by HBM, so:
+//   e4m3: the product in packed BF16, which is exact (a result too small for BF16's
+//   normal range is far below half of e4m3's smallest step);
+//   int8: x inv + 1.5 * 2^23 in one FMA, whose low byte is x inv rounded to nearest even
+//   (the sum's unit in the last place is 1); infinities and NaN go the long way.
+template <bool kInt8>
+__device__ __forceinline__ uint2 quantize8(uint4 v, float inv, bool finite) {
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  uint32_t o[2];
+  if constexpr (kInt8) {
+    if (finite) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        constexpr float kMagic = 12582912.0f;
+        const uint32_t a = __float_as_uint(fmaf(bf_lo(w[2 * h]), inv, kMagic)), b = __float_as_uint(fmaf(bf_hi(w[2 * h]), inv, kMagic));
+        const uint32_t c = __float_as_uint(fmaf(bf_lo(w[2 * h + 1]), inv, kMagic)), d = __float_as_uint(fmaf(bf_hi(w[2 * h + 1]), inv, kMagic));
+        o[h] = __byte_perm(__byte_perm(a, b, 0x0040), __byte_perm(c, d, 0x0040), 0x5410);
+      }
+    } else {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        o[h] = pack8<true>(bf_lo(w[2 * h]) * inv, bf_hi(w[2 * h]) * inv, bf_lo(w[2 * h + 1]) * inv, bf_hi(w[2 * h + 1]) * inv);
+    }
+  } else {
+    const __nv_bfloat162 f = __float2bfloat162_rn(inv);
+    uint32_t y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const __nv_bfloat162 t = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&w[i]), f);
+      y[i] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) o[h] = pack8<false>(bf_lo(y[2 * h]), bf_hi(y[2 * h]), bf_lo(y[2 * h + 1]), bf_hi(y[2 * h + 1]));
+  }
+  return make_uint2(o[0], o[1]);
+}
 
 struct RowRange {
   int start, end;
@@ -128,7 +186,6 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   const __nv_bfloat16* x = p.x[kv] + b * p.sb[kv] + g * p.sh[kv] + 8 * c;
   uint8_t* cache = p.cache[kv] + unit * p.Smax * 128;
   uint4 v[kPasses];
-  uint32_t amax = 0;
 #pragma unroll
   for (int i = 0; i < kPasses; ++i) {
     const int pos = row0 + 16 * i + (tid >> 4);
@@ -136,8 +193,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     if (pos >= rg.start && pos < rg.end)
       v[i] = *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(pos - rg.start) * p.st[kv]);
   }
-#pragma unroll
-  for (int i = 0; i < kPasses; ++i) amax = max(amax, abs_max_bits(v[i]));
+  bool finite;
+  uint32_t amax = abs_max_bits<kPasses>(v, finite);
   __shared__ uint32_t warp_max[kAppendThreads / 32];
   __shared__ float old_scale_sh;
   float* scale = p.scale[kv] + unit * p.nblk + blk;
@@ -145,8 +202,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   if ((tid & 31) == 0) warp_max[tid >> 5] = amax;
   if (tid == 0) old_scale_sh = *scale;
   __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kAppendThreads / 32; ++w) amax = max(amax, warp_max[w]);
+  amax = __reduce_max_sync(0xffffffffu, warp_max[tid & (kAppendThreads / 32 - 1)]);
   const bool has_old = rg.start > row0;
   const float old_scale = old_scale_sh;
   const float s = grown_scale<kInt8>(amax, has_old, old_scale);
@@ -162,10 +218,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   for (int i = 0; i < kPasses; ++i) {
     const int pos = row0 + 16 * i + (tid >> 4);
     if (pos < rg.start || pos >= rg.end) continue;
-    uint2 o;
-    o.x = pack8<kInt8>(bf_lo(v[i].x) * inv, bf_hi(v[i].x) * inv, bf_lo(v[i].y) * inv, bf_hi(v[i].y) * inv);
-    o.y = pack8<kInt8>(bf_lo(v[i].z) * inv, bf_hi(v[i].z) * inv, bf_lo(v[i].w) * inv, bf_hi(v[i].w) * inv);
-    *reinterpret_cast<uint2*>(cache + static_cast<int64_t>(pos) * 128 + 8 * c) = o;
+    *reinterpret_cast<uint2*>(cache + static_cast<int64_t>(pos) * 128 + 8 * c) = quantize8<kInt8>(v[i], inv, finite);
   }
   if (tid == 0) *scale = s;
   if (kv == 0 && p.weights != nullptr && tid < kBlock) {
