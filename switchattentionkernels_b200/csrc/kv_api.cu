@@ -44,7 +44,7 @@ int check_cache(int dtype, int B, int Hkv, int Smax, int block) {
 struct KvDecodePlan {
   int heads, nhb, ctas;
   int64_t slots, tiles;
-  size_t cum, cta_status, ml, o, scores, bytes;  // offsets of the workspace's parts, and its size
+  size_t share, cta_status, ml, o, scores, bytes;  // offsets of the workspace's parts, and its size
 };
 
 KvDecodePlan plan_decode(int B, int Smax, int Hq, int Hkv, bool weights, int nsm) {
@@ -57,8 +57,8 @@ KvDecodePlan plan_decode(int B, int Smax, int Hq, int Hkv, bool weights, int nsm
   d.ctas = static_cast<int>(std::min<int64_t>(d.tiles, static_cast<int64_t>(nsm) * swa::kKvDecodeCtasPerSm));
   d.slots = units + d.ctas;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-  d.cum = 256;  // the status word first
-  d.cta_status = up(d.cum + (static_cast<size_t>(B) + 1) * 4);
+  d.share = 256;  // the status word first
+  d.cta_status = up(d.share + static_cast<size_t>(d.ctas) * 16);
   d.ml = up(d.cta_status + static_cast<size_t>(d.ctas) * 4);
   d.o = up(d.ml + static_cast<size_t>(d.slots) * d.heads * 8);
   d.scores = up(d.o + static_cast<size_t>(d.slots) * d.heads * 512);
@@ -86,6 +86,9 @@ int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
       return fail(SWA_E_INVALID, "strides of k/v must be multiples of 8 elements");
+  for (const int32_t* t : {start, new_lens})
+    if (t != nullptr && t != seq_lens && t < seq_lens + B && seq_lens < t + B)
+      return fail(SWA_E_INVALID, "start and new_lens may be seq_lens but not overlap it otherwise");
   if (T > 1 && (B > 65535 || 2 * static_cast<int64_t>(Hkv) > 65535))
     return fail(SWA_E_UNSUPPORTED, "append grid: at most 65535 sequences and 32767 KV heads");
   int nsm = 0;
@@ -108,6 +111,7 @@ int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides
   p.start = start;
   p.new_lens = new_lens;
   p.seq_lens = seq_lens;
+  p.lens_after = start == seq_lens || new_lens == seq_lens;
   p.B = B;
   p.T = T;
   p.Hkv = Hkv;
@@ -173,7 +177,7 @@ int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const v
   p.weights = key_weights;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.status = reinterpret_cast<int32_t*>(ws);
-  p.cum = reinterpret_cast<int32_t*>(ws + d.cum);
+  p.share = reinterpret_cast<int4*>(ws + d.share);
   p.cta_status = reinterpret_cast<int32_t*>(ws + d.cta_status);
   p.part_ml = reinterpret_cast<float*>(ws + d.ml);
   p.part_o = reinterpret_cast<float*>(ws + d.o);

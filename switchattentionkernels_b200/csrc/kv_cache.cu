@@ -177,6 +177,8 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
   constexpr int kBlock = 16 * kPasses;
   const int b = blockIdx.z, g = blockIdx.y >> 1, kv = blockIdx.y & 1;
   const RowRange rg = append_range(p, b);
+  cudaTriggerProgrammaticLaunchCompletion();
+  if (!p.lens_after && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.seq_lens[b] = rg.end;
   const int blk = rg.start / kBlock + blockIdx.x;
   const int row0 = blk * kBlock;
   if (rg.end <= rg.start || row0 >= rg.end) return;
@@ -228,6 +230,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
 }
 
 __global__ void kv_advance_kernel(const __grid_constant__ KvAppendParams p) {
+  cudaGridDependencySynchronize();  // the append has read the old lengths
   const int b = blockIdx.x * blockDim.x + threadIdx.x;
   if (b < p.B) p.seq_lens[b] = append_range(p, b).end;
 }
@@ -284,8 +287,8 @@ cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
   }
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
-  kv_advance_kernel<<<(p.B + 127) / 128, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  if (!p.lens_after) return cudaSuccess;
+  return launch_dependent(kv_advance_kernel, dim3((p.B + 127) / 128), dim3(128), stream, p);
 }
 
 // ---------------------------------------------------------------------------

@@ -14,6 +14,23 @@
 
 namespace swa {
 
+// Launches `kernel` as the dependent of the kernel before it on the stream: its CTAs may
+// start while that one still runs, and wait (cudaGridDependencySynchronize) for its
+// end before they read what it wrote.
+template <typename... Params, typename... Args>
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Args&&>(args)...);
+}
+
 struct KvAppendParams {
   const __nv_bfloat16* x[2];  // new K, V rows: element (b, t, g, d) at b * sb + t * st + g * sh + d
   int64_t sb[2], st[2], sh[2];
@@ -23,6 +40,7 @@ struct KvAppendParams {
   const int32_t* start;       // [B] rows already cached (may be seq_lens)
   const int32_t* new_lens;    // [B] new rows of each sequence, or null: T
   int32_t* seq_lens;          // [B] written: rows cached after the call
+  bool lens_after;            // start (or new_lens) is seq_lens: written once every CTA has read it
   int B, T, Hkv, Smax, nblk, block;
 };
 cudaError_t launch_kv_append(const KvAppendParams& p, bool int8, cudaStream_t stream);
@@ -58,7 +76,7 @@ struct __align__(64) KvDecodeParams {
   float* lse;                 // [B, Hq]
   float* weights;             // [B, Hkv, Smax] added to, or null
   // workspace
-  int32_t* cum;               // [B + 1] tiles of one head of the sequences before b
+  int4* share;                // [ctas] {unit of the first tile, that tile's index in it, tiles, tiles of the unit}
   int32_t* cta_status;        // [ctas]
   int32_t* status;
   float* part_ml;             // [slots, heads, 2] maximum and sum of each partial row

@@ -198,6 +198,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   const int cta = blockIdx.x;
   const int units = p.Hkv * p.nhb;  // units of a sequence
 
+  cudaTriggerProgrammaticLaunchCompletion();  // the second kernel waits for this one's end by itself
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 1);
@@ -242,18 +243,12 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       if (w < warp) before += scan[w];
       total += scan[w];
     }
-    if (cta == 0) {
-      int c = before;
-      for (int b = b0; b < b1; ++b) {
-        p.cum[b] = c;
-        c += seq_tiles(p, b);
-      }
-      if (tid == 0) p.cum[p.B] = total;
-    }
     const int tiles = total * units;
     const int per = (tiles + p.ctas - 1) / p.ctas;
     const int t0 = cta * per, t1 = min(tiles, t0 + per);
-    if (t0 < t1 && t0 >= before * units && t0 < (before + sum) * units) {  // exactly one thread
+    if (t0 >= t1) {
+      if (tid == 0) p.share[cta] = make_int4(0, 0, 0, 0);
+    } else if (t0 >= before * units && t0 < (before + sum) * units) {  // exactly one thread
       int b = b0, c = before * units;
       for (;; ++b) {
         const int nb = seq_tiles(p, b) * units;
@@ -266,6 +261,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       share[2] = (t0 - c) % nb;
       share[3] = t1 - t0;
       share[4] = t0;
+      p.share[cta] = make_int4(b * units + share[1], share[2], t1 - t0, nb);
     }
   }
   if (warp == 5) {
@@ -597,128 +593,110 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   if (tid == 0) p.cta_status[cta] = *abort_flag ? kStatusTimeout : 0;
 }
 
-// Second kernel.  Blocks [0, B Hq): one query head each, the merge of its unit's
-// segments (nothing where one CTA did the whole unit).  Blocks from there on (with
-// weights): an equal share of the (sequence, KV head, tile) items each, the weights
-// 2^(s - lse) of a tile's keys summed over the group's heads in a fixed order and
-// added to the accumulated ones.
-constexpr int kMaxCtas = 1024;
-
-struct UnitSplit {
-  int first, last;  // CTAs that worked on the unit
-};
-__device__ __forceinline__ UnitSplit unit_split(const KvDecodeParams& p, int b, int u, int n) {
+// Second kernel, one block of 128 threads per head of a head block for each CTA of the
+// first.  blockIdx.y = 0: where CTA c's share begins inside a unit that the CTA before
+// began, the block merges that unit's segments; the blocks also write the rows of
+// sequences without a key.  blockIdx.y >= 1 (with weights): the attention weights
+// 2^(s - lse) of the keys of CTA c's tiles, summed over the group's heads in a fixed
+// order and added to the accumulated ones, kHeads tiles at a time.
+template <int kHeads, bool kWeights>
+__global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
+  __shared__ float lse_sh[kHeads];
+  const int tid = threadIdx.x & 127, h = threadIdx.x >> 7, lane = threadIdx.x & 31;
+  const int c = blockIdx.x;
   const int units = p.Hkv * p.nhb;
-  const int tiles = p.cum[p.B] * units;
-  const int per = (tiles + p.ctas - 1) / p.ctas;
-  const int t0 = p.cum[b] * units + u * n;
-  return UnitSplit{t0 / per, (t0 + n - 1) / per};
-}
-
-__global__ void __launch_bounds__(128) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
-  __shared__ float wsh[kMaxCtas];
-  __shared__ float red[8];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int units = p.Hkv * p.nhb;
-  if (blockIdx.x == 0) {
-    int st = 0;
-    for (int c = tid; c < p.ctas; c += 128) st |= p.cta_status[c];
-    st = __syncthreads_or(st);
-    if (tid == 0) *p.status = st != 0 ? kStatusTimeout : 0;
-  }
-  const int n_heads = p.B * p.Hq;
-  if (static_cast<int>(blockIdx.x) < n_heads) {
-    const int b = blockIdx.x / p.Hq, hq = blockIdx.x % p.Hq;
-    const int hr = hq % p.r;
-    const int u = (hq / p.r) * p.nhb + hr / p.heads, h = hr % p.heads;
-    const int n = p.cum[b + 1] - p.cum[b];
-    const int64_t row = blockIdx.x;
-    if (n == 0) {  // no key: 0 / 0 and log2 0, as the prefill writes a row without a legal key
-      p.out[row * 128 + tid] = __float2bfloat16_rn(__uint_as_float(0x7FC00000u));
-      if (tid == 0) p.lse[row] = -INFINITY;
-      return;
+  cudaGridDependencySynchronize();
+  const int4 sh = p.share[c];
+  const int per = p.share[0].z;  // tiles of every CTA but the last ones
+  if (blockIdx.y == 0) {
+    if (c == 0) {
+      int st = 0;
+      for (int i = threadIdx.x; i < p.ctas; i += 128 * kHeads) st |= p.cta_status[i];
+      st = __syncthreads_or(st);
+      if (threadIdx.x == 0) *p.status = st != 0 ? kStatusTimeout : 0;
     }
-    const UnitSplit us = unit_split(p, b, u, n);
-    if (us.first == us.last) return;
-    const int nseg = us.last - us.first + 1;
-    const int64_t slot0 = static_cast<int64_t>(b) * units + u + us.first;
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * p.heads + h;
-    float M = -INFINITY;
-    for (int i = tid; i < nseg; i += 128) M = fmaxf(M, ml[static_cast<int64_t>(i) * p.heads].x);
+    for (int b = c; b < p.B; b += p.ctas) {
+      if (p.seq_lens[b] > 0) continue;
+      // no key: 0 / 0 and log2 0, as the prefill writes a row without a legal key
+      for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.Hq) * 128; i += 128 * kHeads)
+        p.out[static_cast<int64_t>(b) * p.Hq * 128 + i] = __float2bfloat16_rn(__uint_as_float(0x7FC00000u));
+      for (int i = threadIdx.x; i < p.Hq; i += 128 * kHeads) p.lse[static_cast<int64_t>(b) * p.Hq + i] = -INFINITY;
+    }
+    // sh.y tiles of the unit lie before this CTA's: the CTA before began it if it holds them all
+    if (sh.z == 0 || sh.y == 0 || sh.y > per) return;
+    const int b = sh.x / units, u = sh.x % units;
+    const int hb = u % p.nhb;
+    if (h >= min(kHeads, p.r - hb * kHeads)) return;
+    const int first = c - 1, last = (c * per - sh.y + sh.w - 1) / per;
+    const int nseg = last - first + 1;
+    const int64_t slot0 = static_cast<int64_t>(sh.x) + first;
+    const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
+    float M = -INFINITY, L = 0.0f;
+    for (int i = lane; i < nseg; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * kHeads].x);
     M = warp_max(M);
-    if (lane == 0) red[warp] = M;
-    __syncthreads();
-    M = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    float L = 0.0f;
-    for (int i = tid; i < nseg; i += 128) {
-      const float2 x = ml[static_cast<int64_t>(i) * p.heads];
-      const float w = ex2_approx(x.x - M);
-      wsh[i] = w;
-      L = fmaf(x.y, w, L);
-    }
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-    if (lane == 0) red[4 + warp] = L;
-    __syncthreads();
-    L = (red[4] + red[5]) + (red[6] + red[7]);
-    const float* po = p.part_o + (slot0 * p.heads + h) * 128 + tid;
+    const float* po = p.part_o + (slot0 * kHeads + h) * 128 + tid;
     float acc = 0.0f;
 #pragma unroll 8
-    for (int i = 0; i < nseg; ++i) acc = fmaf(po[static_cast<int64_t>(i) * p.heads * 128], wsh[i], acc);
+    for (int i = 0; i < nseg; ++i) {
+      const float2 x = ml[static_cast<int64_t>(i) * kHeads];
+      const float w = ex2_approx(x.x - M);
+      L = fmaf(x.y, w, L);
+      acc = fmaf(po[static_cast<int64_t>(i) * kHeads * 128], w, acc);
+    }
+    const int64_t row = static_cast<int64_t>(b) * p.Hq + (u / p.nhb) * p.r + hb * kHeads + h;
     p.out[row * 128 + tid] = __float2bfloat16_rn(acc / L);
     if (tid == 0) p.lse[row] = lg2_approx(L) + M;
     return;
   }
-  // accumulated weights
-  const int share = gridDim.x - n_heads, me = blockIdx.x - n_heads;
-  const int items = p.cum[p.B] * p.Hkv;
-  const int per = (items + share - 1) / share;
-  int t = me * per;
-  const int t1 = min(items, t + per);
-  if (t >= t1) return;
-  int b = 0, last = p.B;  // cum[b] Hkv <= t < cum[b + 1] Hkv
-  while (last - b > 1) {
-    const int mid = (b + last) / 2;
-    if (p.cum[mid] * p.Hkv <= t) b = mid; else last = mid;
-  }
-  while (t < t1) {
-    while (p.cum[b + 1] * p.Hkv <= t) ++b;
-    const int n = p.cum[b + 1] - p.cum[b];
-    const int g = (t - p.cum[b] * p.Hkv) / n;
-    const int i0 = t - p.cum[b] * p.Hkv - g * n;
-    const int cnt = min(n - i0, t1 - t);
-    const KeyRange kr = key_range(p, b);
-    float* dst = p.weights + (static_cast<int64_t>(b) * p.Hkv + g) * p.Smax;
-    for (int hb = 0; hb < p.nhb; ++hb) {
-      const int u = g * p.nhb + hb;
-      const int nh = min(p.heads, p.r - hb * p.heads);
-      const UnitSplit us = unit_split(p, b, u, n);
-      const int nseg = us.last - us.first + 1;
-      const int64_t slot0 = static_cast<int64_t>(b) * units + u + us.first;
-      __syncthreads();
-      for (int h = warp; h < nh; h += 4) {  // lse of each head from its segments
-        const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * p.heads + h;
-        float M = -INFINITY, L = 0.0f;
-        for (int i = lane; i < nseg; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * p.heads].x);
-        M = warp_max(M);
-        for (int i = lane; i < nseg; i += 32) {
-          const float2 x = ml[static_cast<int64_t>(i) * p.heads];
-          L = fmaf(x.y, ex2_approx(x.x - M), L);
-        }
+  if constexpr (kWeights) {
+    if (sh.z == 0) return;
+    Segments seg{};
+    seg.b = sh.x / units;
+    seg.u = sh.x % units;
+    seg.off = sh.y;
+    seg.left = sh.z;
+    int t = c * per;  // first tile of the segment, of the whole batch
+    while (seg.next(p)) {
+      const int g = seg.cur_u / p.nhb, hb0 = seg.cur_u % p.nhb;
+      if (hb0 == 0) {  // a key's tile of the first head block stands for its tiles of the others
+        float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
+        for (int hb = 0; hb < p.nhb; ++hb) {
+          const int nh = min(kHeads, p.r - hb * kHeads);
+          const int t0 = t - seg.first + hb * seg.all;  // first tile of the unit
+          const int first = t0 / per, last = (t0 + seg.all - 1) / per;
+          const int64_t slot0 = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first;
+          __syncthreads();
+          if ((threadIdx.x & 96) == 0 && h < nh) {  // the head's lse from its segments
+            const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
+            float M = -INFINITY, L = 0.0f;
+            for (int i = lane; i <= last - first; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * kHeads].x);
+            M = warp_max(M);
+            for (int i = lane; i <= last - first; i += 32) {
+              const float2 x = ml[static_cast<int64_t>(i) * kHeads];
+              L = fmaf(x.y, ex2_approx(x.x - M), L);
+            }
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-        if (lane == 0) red[h] = lg2_approx(L) + M;
+            for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
+            if (lane == 0) lse_sh[h] = lg2_approx(L) + M;
+          }
+          __syncthreads();
+          const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + tid;
+          for (int i = h + kHeads * (blockIdx.y - 1); i < seg.n; i += kHeads * (gridDim.y - 1)) {
+            const int key = seg.lo + (seg.first + i) * kTile + tid;
+            if (key >= seg.hi) continue;
+            const float before = dst[key];
+            float s[kHeads];
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) s[j] = j < nh ? sc[(static_cast<int64_t>(i) * kHeads + j) * kTile] : 0.0f;
+            float w = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kHeads; ++j) w += j < nh ? ex2_approx(s[j] - lse_sh[j]) : 0.0f;
+            dst[key] = before + w;
+          }
+        }
       }
-      __syncthreads();
-      const float* sc = p.scores + (static_cast<int64_t>(p.cum[b]) * units + static_cast<int64_t>(u) * n + i0) * p.heads * kTile + tid;
-      for (int i = 0; i < cnt; ++i) {
-        const int key = kr.lo + (i0 + i) * kTile + tid;
-        float w = 0.0f;
-        for (int h = 0; h < nh; ++h) w += ex2_approx(sc[(static_cast<int64_t>(i) * p.heads + h) * kTile] - red[h]);
-        if (key < kr.hi) dst[key] += w;
-      }
+      t += seg.n;
     }
-    t += cnt;
   }
 }
 
@@ -735,7 +713,9 @@ cudaError_t launch_main(const KvDecodeParams& p, cudaStream_t stream) {
     if (dev < 64) attr_set[dev] = true;
   }
   kv_decode_kernel<kInt8, kHeads, kWeights><<<p.ctas, kThreads, KvSmem<kHeads>::bytes, stream>>>(p);
-  return cudaGetLastError();
+  e = cudaGetLastError();
+  if (e != cudaSuccess) return e;
+  return launch_dependent(kv_decode_merge_kernel<kHeads, kWeights>, dim3(p.ctas, kWeights ? 2 : 1), dim3(128 * kHeads), stream, p);
 }
 
 template <bool kInt8>
@@ -748,11 +728,7 @@ cudaError_t launch_for(const KvDecodeParams& p, cudaStream_t stream) {
 }  // namespace
 
 cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream) {
-  cudaError_t e = int8 ? launch_for<true>(p, stream) : launch_for<false>(p, stream);
-  if (e != cudaSuccess) return e;
-  const int extra = p.weights != nullptr ? p.ctas : 0;
-  kv_decode_merge_kernel<<<p.B * p.Hq + extra, 128, 0, stream>>>(p);
-  return cudaGetLastError();
+  return int8 ? launch_for<true>(p, stream) : launch_for<false>(p, stream);
 }
 
 }  // namespace swa
