@@ -1,5 +1,6 @@
 // C ABI of the block-scaled 8-bit KV cache (declared in include/swattn_b200.h).
 #include <algorithm>
+#include <atomic>
 #include <string>
 
 #include "../../include/swattn_b200.h"
@@ -18,14 +19,19 @@ int cuda_fail(cudaError_t e, const char* what) {
 }
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 
+// SMs of the current device, asked once for each device.
 int device_sms(int* nsm) {
+  static std::atomic<int> known[64];
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
+  if (dev < 64 && (*nsm = known[dev].load(std::memory_order_relaxed)) > 0) return SWA_OK;
   int major = 0;
-  cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
-  cudaDeviceGetAttribute(nsm, cudaDevAttrMultiProcessorCount, dev);
+  e = cudaDeviceGetAttribute(&major, cudaDevAttrComputeCapabilityMajor, dev);
+  if (e == cudaSuccess) e = cudaDeviceGetAttribute(nsm, cudaDevAttrMultiProcessorCount, dev);
+  if (e != cudaSuccess) return cuda_fail(e, "cudaDeviceGetAttribute");
   if (major != 10) return fail(SWA_E_UNSUPPORTED, "this library targets sm_100 (B200) devices");
+  if (dev < 64) known[dev].store(*nsm, std::memory_order_relaxed);
   return SWA_OK;
 }
 

@@ -18,7 +18,9 @@ never synchronise and can be captured into a CUDA graph.
 from __future__ import annotations
 
 import ctypes
+from contextlib import nullcontext
 from dataclasses import dataclass
+from functools import lru_cache
 
 import torch
 
@@ -27,6 +29,7 @@ from ._core import LOG2E
 
 HEAD_DIM = 128
 BLOCK_SIZES = (16, 32, 64, 128)
+_Strides = ctypes.c_int64 * 3
 _DTYPES = {torch.float8_e4m3fn: _native.KV_E4M3, torch.int8: _native.KV_INT8}
 
 
@@ -64,8 +67,12 @@ def make_switch_kv_cache(batch: int, max_len: int, kv_heads: int, *, device, dty
                          weights, block_size)
 
 
-def _check_cache(cache: SwitchKVCache, name: str = "cache") -> tuple[int, int, int]:
-    """``(B, Hkv, Smax)`` of a well-formed cache."""
+def _bad(name: str, field: str, dtype, shape) -> ValueError:
+    return ValueError(f"{name}.{field} must be a contiguous {dtype} {list(shape)} tensor on the device of {name}.k")
+
+
+def _check_cache(cache: SwitchKVCache, name: str = "cache") -> tuple[int, int, int, torch.device]:
+    """``(B, Hkv, Smax, device)`` of a well-formed cache."""
     if not isinstance(cache, SwitchKVCache):
         raise TypeError(f"{name} must be a SwitchKVCache")
     k, v = cache.k, cache.v
@@ -73,45 +80,79 @@ def _check_cache(cache: SwitchKVCache, name: str = "cache") -> tuple[int, int, i
         raise TypeError(f"{name}.k must be a device-resident float8_e4m3fn or int8 tensor")
     if not isinstance(v, torch.Tensor) or v.dtype != k.dtype or not v.is_cuda:
         raise TypeError(f"{name}.v must be a device-resident tensor of {name}.k's dtype")
-    if k.ndim != 4 or v.shape != k.shape:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape:
         raise ValueError(f"{name}.k and {name}.v must be [B, Hkv, Smax, 128]")
-    B, Hkv, Smax, D = k.shape
+    B, Hkv, Smax, D = shape
     if D != HEAD_DIM:
         raise ValueError("head_dim must be 128")
     if B == 0 or Hkv == 0 or Smax == 0:
         raise ValueError(f"{name} is empty")
     if cache.block_size not in BLOCK_SIZES:
         raise ValueError("block_size must be 16, 32, 64 or 128")
-    blocks = -(-Smax // cache.block_size)
-    expected = [("v", v, k.dtype, (B, Hkv, Smax, D)), ("k", k, k.dtype, (B, Hkv, Smax, D)),
-                ("k_scale", cache.k_scale, torch.float32, (B, Hkv, blocks)),
-                ("v_scale", cache.v_scale, torch.float32, (B, Hkv, blocks)),
-                ("seq_lens", cache.seq_lens, torch.int32, (B,))]
-    if cache.key_weights is not None:
-        expected.append(("key_weights", cache.key_weights, torch.float32, (B, Hkv, Smax)))
-    for field, t, dtype, shape in expected:
-        if (not isinstance(t, torch.Tensor) or t.dtype != dtype or tuple(t.shape) != shape or t.device != k.device
+    dev = k.device
+    if not k.is_contiguous():
+        raise _bad(name, "k", k.dtype, shape)
+    if not v.is_contiguous() or v.device != dev:
+        raise _bad(name, "v", k.dtype, shape)
+    scales = (B, Hkv, -(-Smax // cache.block_size))
+    for field, t in (("k_scale", cache.k_scale), ("v_scale", cache.v_scale)):
+        if (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != scales or t.device != dev
                 or not t.is_contiguous()):
-            raise ValueError(f"{name}.{field} must be a contiguous {dtype} {list(shape)} tensor on the device of {name}.k")
-    return B, Hkv, Smax
+            raise _bad(name, field, torch.float32, scales)
+    t = cache.seq_lens
+    if (not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.shape != (B,) or t.device != dev
+            or not t.is_contiguous()):
+        raise _bad(name, "seq_lens", torch.int32, (B,))
+    t = cache.key_weights
+    if t is not None and (not isinstance(t, torch.Tensor) or t.dtype != torch.float32 or t.shape != (B, Hkv, Smax)
+                          or t.device != dev or not t.is_contiguous()):
+        raise _bad(name, "key_weights", torch.float32, (B, Hkv, Smax))
+    return B, Hkv, Smax, dev
 
 
-def _check_rows(t, name: str, shape: tuple, dev) -> None:
+def _check_rows(t, name: str, shape: tuple, dev) -> tuple:
+    """The strides of BF16 rows of ``shape``."""
     if not isinstance(t, torch.Tensor) or t.dtype != torch.bfloat16 or not t.is_cuda:
         raise TypeError(f"{name} must be a device-resident bfloat16 tensor")
     if t.device != dev:
         raise ValueError(f"{name} must be on the device of the cache")
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}")
     # a slice of a fused projection is fine: only the 128 values of a row have to lie together
-    if t.stride(-1) != 1 or any(s % 8 for s in t.stride()[:-1]) or t.data_ptr() % 16:
+    st = t.stride()
+    bits = t.data_ptr() >> 1
+    for s in st[:-1]:
+        bits |= s
+    if st[-1] != 1 or bits & 7:
         raise ValueError(f"{name} needs contiguous, 16-byte aligned rows (other strides multiples of 8 elements)")
+    return st
 
 
-def _check_lens(t, name: str, B: int, dev) -> None:
-    if (not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32 or tuple(t.shape) != (B,)
+def _check_lens(t, name: str, B: int, dev) -> int:
+    if (not isinstance(t, torch.Tensor) or t.device != dev or t.dtype != torch.int32 or t.shape != (B,)
             or not t.is_contiguous()):
         raise ValueError(f"{name} must be a contiguous int32 [B] tensor on the device of the cache")
+    return t.data_ptr()
+
+
+def _on(dev: torch.device):
+    """Makes ``dev`` the current device for the calls inside (nothing to do where it is)."""
+    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+
+
+def _stream(dev: torch.device) -> int:
+    return torch.cuda.current_stream(dev).cuda_stream
+
+
+@lru_cache(maxsize=256)
+def _decode_workspace_bytes(B: int, Smax: int, Hq: int, Hkv: int, weights: bool, device_index: int) -> int:
+    """The decode step's workspace on the current device, ``device_index``: a function of the shapes."""
+    lib = _native.load()
+    nbytes = int(lib.swa_kv_decode_workspace_bytes(B, Smax, Hq, Hkv, int(weights)))
+    if nbytes <= 0:
+        raise RuntimeError("decode workspace size query failed: " + lib.swa_last_error_string().decode(errors="replace"))
+    return nbytes
 
 
 def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: torch.Tensor, *,
@@ -130,34 +171,28 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     even; infinities saturate and do not count for the scale, NaN stays NaN in an e4m3
     cache and becomes 0 in an int8 one.  Appended rows start with ``key_weights`` 0.
     """
-    B, Hkv, Smax = _check_cache(cache)
-    dev = cache.k.device
-    token = isinstance(k_new, torch.Tensor) and k_new.ndim == 3
+    B, Hkv, Smax, dev = _check_cache(cache)
     if not isinstance(k_new, torch.Tensor) or k_new.ndim not in (3, 4):
         raise ValueError("k_new must have shape [B, T, Hkv, 128] or [B, Hkv, 128]")
+    token = k_new.ndim == 3
     T = 1 if token else int(k_new.shape[1])
     shape = (B, Hkv, HEAD_DIM) if token else (B, T, Hkv, HEAD_DIM)
-    _check_rows(k_new, "k_new", shape, dev)
-    _check_rows(v_new, "v_new", shape, dev)
-    if new_lens is not None:
-        _check_lens(new_lens, "new_lens", B, dev)
-    if start is None:
-        start = cache.seq_lens
-    else:
-        _check_lens(start, "start", B, dev)
+    strides = []
+    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
+        st = _check_rows(t, name, shape, dev)
+        strides.append(_Strides(st[0], 0, st[1]) if token else _Strides(st[0], st[1], st[2]))
+    lens_ptr = None if new_lens is None else _check_lens(new_lens, "new_lens", B, dev)
+    seq_ptr = cache.seq_lens.data_ptr()
+    start_ptr = seq_ptr if start is None else _check_lens(start, "start", B, dev)
     if T == 0:
         return
-    strides = []
-    for t in (k_new, v_new):
-        st = t.stride()
-        strides.append((ctypes.c_int64 * 3)(st[0], 0 if token else st[1], st[1] if token else st[2]))
-    lib = _native.load()
-    with torch.cuda.device(dev):
-        rc = lib.swa_kv_append(_native.ptr(k_new), _native.ptr(v_new), strides[0], strides[1], _native.ptr(start),
-                               _native.ptr(new_lens), _native.ptr(cache.k), _native.ptr(cache.v),
-                               _native.ptr(cache.k_scale), _native.ptr(cache.v_scale),
-                               _native.ptr(cache.key_weights), _native.ptr(cache.seq_lens), B, T, Hkv, Smax, HEAD_DIM,
-                               cache.block_size, _DTYPES[cache.k.dtype], _native.stream_ptr(dev))
+    weights = cache.key_weights
+    with _on(dev):
+        rc = _native.load().swa_kv_append(
+            k_new.data_ptr(), v_new.data_ptr(), strides[0], strides[1], start_ptr, lens_ptr, cache.k.data_ptr(),
+            cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+            None if weights is None else weights.data_ptr(), seq_ptr, B, T, Hkv, Smax, HEAD_DIM, cache.block_size,
+            _DTYPES[cache.k.dtype], _stream(dev))
     _native.check(rc, "switch_kv_cache_append")
 
 
@@ -177,8 +212,7 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
     row that was attended to, summed over the query heads of its KV head, is added to
     them.  ``status_out``: as in ``switch_gqa_decode_forward``.
     """
-    B, Hkv, Smax = _check_cache(cache)
-    dev = cache.k.device
+    B, Hkv, Smax, dev = _check_cache(cache)
     squeeze = isinstance(q, torch.Tensor) and q.ndim == 4
     if squeeze:
         if q.shape[1] != 1:
@@ -187,34 +221,30 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
     if not isinstance(q, torch.Tensor) or q.ndim != 3:
         raise ValueError("q must have shape [B, Hq, 128] or [B, 1, Hq, 128]")
     Hq = int(q.shape[1])
-    _check_rows(q, "q", (B, Hq, HEAD_DIM), dev)
+    st = _check_rows(q, "q", (B, Hq, HEAD_DIM), dev)
     if Hq == 0 or Hq % Hkv != 0:
         raise ValueError("query heads must be divisible by KV heads")
     if window_size <= 0:
         raise ValueError("window_size must be positive")
     if (not isinstance(route_full, torch.Tensor) or route_full.device != dev or route_full.dtype != torch.bool
-            or tuple(route_full.shape) != (B,)):
+            or route_full.shape != (B,)):
         raise ValueError("route_full must be a bool [B] tensor on the device of the cache")
     scale = (sm_scale if sm_scale is not None else (1.0 / HEAD_DIM) ** 0.5) * LOG2E
     if not scale > 0:
         raise ValueError("sm_scale must be positive")
     _core._check_status_out(status_out, dev)
     weights = cache.key_weights if accumulate else None
-    lib = _native.load()
     out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
     lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
-    with torch.cuda.device(dev):
-        nbytes = int(lib.swa_kv_decode_workspace_bytes(B, Smax, Hq, Hkv, int(weights is not None)))
-        if nbytes <= 0:
-            raise RuntimeError("decode workspace size query failed: " +
-                               lib.swa_last_error_string().decode(errors="replace"))
+    with _on(dev):
+        nbytes = _decode_workspace_bytes(B, Smax, Hq, Hkv, weights is not None, dev.index)
         ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.int32, device=dev)
-        route = route_full.contiguous().view(torch.uint8)
-        rc = lib.swa_kv_decode(_native.ptr(q), q.stride(0), q.stride(1), _native.ptr(cache.k), _native.ptr(cache.v),
-                               _native.ptr(cache.k_scale), _native.ptr(cache.v_scale), _native.ptr(cache.seq_lens),
-                               _native.ptr(route), _native.ptr(out), _native.ptr(lse), _native.ptr(weights), B, Smax,
-                               Hq, Hkv, HEAD_DIM, cache.block_size, min(int(window_size), Smax), float(scale),
-                               _DTYPES[cache.k.dtype], _native.ptr(ws), ws.numel() * 4, _native.stream_ptr(dev))
+        route = route_full if route_full.is_contiguous() else route_full.contiguous()
+        rc = _native.load().swa_kv_decode(
+            q.data_ptr(), st[0], st[1], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
+            cache.v_scale.data_ptr(), cache.seq_lens.data_ptr(), route.data_ptr(), out.data_ptr(), lse.data_ptr(),
+            None if weights is None else weights.data_ptr(), B, Smax, Hq, Hkv, HEAD_DIM, cache.block_size,
+            min(int(window_size), Smax), float(scale), _DTYPES[cache.k.dtype], ws.data_ptr(), nbytes, _stream(dev))
     _native.check(rc, "switch_gqa_decode_cached")
     if status_out is not None or _core.CHECK_DEVICE_STATUS:
         _core.publish_status(ws[0:1], status_out)
@@ -239,8 +269,7 @@ def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, rec
     that takes the result; ``cache`` is then left as it is.  Returns int32
     ``[B, Hkv, min(keep, Smax)]``: the former row of each kept row, -1 past the last one.
     """
-    B, Hkv, Smax = _check_cache(cache)
-    dev = cache.k.device
+    B, Hkv, Smax, dev = _check_cache(cache)
     if cache.key_weights is None:
         raise ValueError("eviction needs a cache with key_weights")
     keep, sink, recent = int(keep), int(sink), int(recent)
@@ -248,38 +277,39 @@ def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, rec
         raise ValueError("keep must be positive and at least sink + recent, both non-negative")
     if keep >= Smax:  # no sequence is longer
         keep, sink, recent = Smax, 0, 0
-    n = keep
-    dst = cache
+    src = _pointers(cache)
+    dst, So = src, Smax
     if out is not None and out is not cache:
-        Bo, Ho, So = _check_cache(out, "out")
+        Bo, Ho, So, dev_out = _check_cache(out, "out")
         if (Bo, Ho) != (B, Hkv) or out.k.dtype != cache.k.dtype or out.block_size != cache.block_size:
             raise ValueError("out must have the batch, heads, dtype and block size of the cache")
-        if out.k.device != dev:
+        if dev_out != dev:
             raise ValueError("out must be on the device of the cache")
         if out.key_weights is None:
             raise ValueError("out must have key_weights")
-        if So < n:
+        if So < keep:
             raise ValueError("out holds fewer rows than are kept")
-        mine = [_extent(t) for t in _tensors(cache)]
-        if any(a0 < b1 and b0 < a1 for a0, a1 in (_extent(t) for t in _tensors(out)) for b0, b1 in mine):
-            raise ValueError("out must not share memory with the cache")
-        dst = out
-    slots = torch.empty((B, Hkv, n), dtype=torch.int32, device=dev)
-    lib = _native.load()
-    with torch.cuda.device(dev):
-        rc = lib.swa_kv_evict(_native.ptr(cache.k), _native.ptr(cache.v), _native.ptr(cache.k_scale),
-                              _native.ptr(cache.v_scale), _native.ptr(cache.key_weights), _native.ptr(cache.seq_lens),
-                              _native.ptr(dst.k), _native.ptr(dst.v), _native.ptr(dst.k_scale),
-                              _native.ptr(dst.v_scale), _native.ptr(dst.key_weights), _native.ptr(dst.seq_lens),
-                              _native.ptr(slots), B, Hkv, Smax, int(dst.k.shape[2]), HEAD_DIM, cache.block_size, keep,
-                              sink, recent, _DTYPES[cache.k.dtype], _native.stream_ptr(dev))
+        dst = _pointers(out)
+        ends = [0, 0]  # of the cache's and of out's memory up to here, by address
+        for first, end, owner in sorted(_spans(cache, src, 0) + _spans(out, dst, 1)):
+            if first < ends[1 - owner]:
+                raise ValueError("out must not share memory with the cache")
+            ends[owner] = max(ends[owner], end)
+    slots = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    with _on(dev):
+        rc = _native.load().swa_kv_evict(*src, *dst, slots.data_ptr(), B, Hkv, Smax, So, HEAD_DIM, cache.block_size,
+                                         keep, sink, recent, _DTYPES[cache.k.dtype], _stream(dev))
     _native.check(rc, "switch_kv_cache_evict")
     return slots
 
 
-def _tensors(cache: SwitchKVCache):
-    return (cache.k, cache.v, cache.k_scale, cache.v_scale, cache.seq_lens, cache.key_weights)
+def _pointers(c: SwitchKVCache) -> tuple:
+    return (c.k.data_ptr(), c.v.data_ptr(), c.k_scale.data_ptr(), c.v_scale.data_ptr(), c.key_weights.data_ptr(),
+            c.seq_lens.data_ptr())
 
 
-def _extent(t: torch.Tensor) -> tuple[int, int]:
-    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+def _spans(c: SwitchKVCache, ptrs: tuple, owner: int) -> list:
+    """``(first byte, end, owner)`` of the cache's tensors."""
+    rows, scales = c.k.numel(), 4 * c.k_scale.numel()
+    sizes = (rows, rows, scales, scales, 4 * c.key_weights.numel(), 4 * c.seq_lens.numel())
+    return [(p, p + n, owner) for p, n in zip(ptrs, sizes)]
