@@ -288,7 +288,7 @@ cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
   cudaError_t e = cudaGetLastError();
   if (e != cudaSuccess) return e;
   if (!p.lens_after) return cudaSuccess;
-  return launch_dependent(kv_advance_kernel, dim3((p.B + 127) / 128), dim3(128), stream, p);
+  return launch_dependent(kv_advance_kernel, dim3((p.B + 127) / 128), dim3(128), 0, stream, p);
 }
 
 // ---------------------------------------------------------------------------

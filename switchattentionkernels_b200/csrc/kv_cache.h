@@ -16,12 +16,15 @@ namespace swa {
 
 // Launches `kernel` as the dependent of the kernel before it on the stream: its CTAs may
 // start while that one still runs, and wait (cudaGridDependencySynchronize) for its
-// end before they read what it wrote.
+// end before they touch global memory.  Every kernel launched this way does so in every
+// CTA, so that its own end implies the end of all kernels before it.
 template <typename... Params, typename... Args>
-cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, cudaStream_t stream, Args&&... args) {
+cudaError_t launch_dependent(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
+                             Args&&... args) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid;
   cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -90,6 +93,9 @@ struct __align__(64) KvDecodeParams {
 };
 cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream);
 // Resident CTAs of the decode kernel per SM (what its shared memory allows).
-constexpr int kKvDecodeCtasPerSm = 2;
+#ifndef SWA_CPS
+#define SWA_CPS 2
+#endif
+constexpr int kKvDecodeCtasPerSm = SWA_CPS;
 
 }  // namespace swa

@@ -32,7 +32,10 @@ namespace {
 
 constexpr int kTile = 128;                 // keys of a tile
 constexpr int kTileBytes = kTile * 128;
-constexpr int kStages = 3;                 // K tiles and V tiles in flight
+#ifndef SWA_ST
+#define SWA_ST 2
+#endif
+constexpr int kStages = SWA_ST;                 // K tiles and V tiles in flight
 constexpr int kThreads = 192;
 constexpr int kParts = 3;
 constexpr float kE4m3Step = 16.0f;         // weight of an e4m3 part against the next
@@ -47,8 +50,8 @@ struct KvSmem {
   static constexpr uint32_t p = q + cols * 128;                    // 2 x [cols][128 B]
   static constexpr uint32_t red = p + 2 * cols * 128;              // [2][4 warps][12] floats
   static constexpr uint32_t lred = red + 2 * 4 * 12 * 4;           // [2][4 warps][8] floats
-  static constexpr uint32_t qf = lred + 2 * 4 * 8 * 4;             // [8] floats
-  static constexpr uint32_t bars = qf + 32;
+  static constexpr uint32_t qf = lred + 2 * 4 * 8 * 4;             // [2][8] floats
+  static constexpr uint32_t bars = qf + 64;
   static constexpr uint32_t misc = bars + 24 * 8;                  // tmem holder, abort flag, start of the share
   static constexpr uint32_t total = misc + 64;
   static constexpr uint32_t bytes = total + 1024;
@@ -78,20 +81,38 @@ __device__ __forceinline__ int seq_tiles(const KvDecodeParams& p, int b) {
 
 // A CTA's share of the tiles, segment by segment.
 struct Segments {
-  int b, u, off, left;  // sequence, unit in it (KV head x head block), first tile in the unit, tiles left
-  // current segment
-  int lo, hi, first, n, all;  // legal keys; first tile, tiles; tiles of the unit
+  int b, u, off, left;  // of the next segment: sequence, unit in it (KV head x head block), first tile; tiles left
+  int lo, hi, all;      // legal keys of sequence b, tiles of its units
+  // the current segment
+  int cur_b, cur_u, cur_lo, cur_hi, cur_all, first, n;
+
+  // share: {sequence, unit, tile, tiles, -, lo, hi, tiles of the unit}
+  __device__ __forceinline__ void start(const int* share) {
+    b = share[0];
+    u = share[1];
+    off = share[2];
+    left = share[3];
+    lo = share[5];
+    hi = share[6];
+    all = share[7];
+  }
+  __device__ __forceinline__ void sequence(const KvDecodeParams& p) {
+    const KeyRange r = key_range(p, b);
+    lo = r.lo;
+    hi = r.hi;
+    all = (r.hi - r.lo + kTile - 1) / kTile;
+  }
   __device__ __forceinline__ bool next(const KvDecodeParams& p) {
     if (left <= 0) return false;
-    for (;; ++b) {  // (only sequences without a key are skipped)
-      const KeyRange r = key_range(p, b);
-      all = (r.hi - r.lo + kTile - 1) / kTile;
-      lo = r.lo;
-      hi = r.hi;
-      if (all > 0) break;
+    while (all == 0) {  // sequences without a key
+      ++b;
+      sequence(p);
     }
     cur_b = b;
     cur_u = u;
+    cur_lo = lo;
+    cur_hi = hi;
+    cur_all = all;
     first = off;
     n = min(all - off, left);
     left -= n;
@@ -101,11 +122,11 @@ struct Segments {
       if (++u == p.Hkv * p.nhb) {
         u = 0;
         ++b;
+        if (left > 0) sequence(p);
       }
     }
     return true;
   }
-  int cur_b, cur_u;
 };
 
 __device__ __forceinline__ float pow2_at_least_448th(float a) {  // smallest 2^e with 448 * 2^e >= a
@@ -193,12 +214,12 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   static_assert(4 * kStages + 4 * 2 + 3 <= 24, "barrier space");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + Sm::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::misc + 4);
-  int* share = reinterpret_cast<int*>(smem + Sm::misc + 8);  // of this CTA: sequence, unit, tile in it, tiles, first tile
+  int* share = reinterpret_cast<int*>(smem + Sm::misc + 8);  // see Segments::start; [4]: first tile of the batch's
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
   const int units = p.Hkv * p.nhb;  // units of a sequence
 
-  cudaTriggerProgrammaticLaunchCompletion();  // the second kernel waits for this one's end by itself
+  // set up what needs no global memory while the kernel before this one ends
   if (tid == 0) {
     for (int s = 0; s < kStages; ++s) {
       mbar_init(&k_full[s], 1);
@@ -219,10 +240,23 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     share[3] = 0;
     fence_barrier_init();
   }
+  if (tid == 128) {
+    tma_prefetch_desc(&p.map[0]);
+    tma_prefetch_desc(&p.map[1]);
+  }
   // unused columns of Q and P are zero
   for (int i = tid; i < 3 * kCols * 8; i += kThreads)
     reinterpret_cast<uint4*>(smem + Sm::q)[i] = make_uint4(0, 0, 0, 0);
   fence_proxy_async_smem();
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();  // the second kernel waits for this one's end by itself
+  // (tensor memory only from here on: a CTA that held some while it waits for the kernel before
+  // could keep that one from getting its own)
+  if (warp == 5) {
+    __syncwarp();
+    tmem_alloc(tmem_holder, 4 * kCols);
+    tmem_relinquish();
+  }
   {
     // this CTA's share: thread t sums the tiles of a run of sequences, then a scan over the threads
     int* scan = reinterpret_cast<int*>(smem + Sm::red);
@@ -261,13 +295,12 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       share[2] = (t0 - c) % nb;
       share[3] = t1 - t0;
       share[4] = t0;
+      const KeyRange kr = key_range(p, b);
+      share[5] = kr.lo;
+      share[6] = kr.hi;
+      share[7] = nb;
       p.share[cta] = make_int4(b * units + share[1], share[2], t1 - t0, nb);
     }
-  }
-  if (warp == 5) {
-    __syncwarp();
-    tmem_alloc(tmem_holder, 4 * kCols);
-    tmem_relinquish();
   }
   tc_fence_before();
   __syncthreads();
@@ -275,16 +308,11 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   const uint32_t tmem = *tmem_holder;  // S: columns 0 and kCols, O: 2 kCols and 3 kCols
   const int ntiles = share[3];
   Segments seg{};
-  seg.b = share[0];
-  seg.u = share[1];
-  seg.off = share[2];
-  seg.left = ntiles;
+  seg.start(share);
 
   if (warp == 4) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0 && ntiles > 0) {
-      tma_prefetch_desc(&p.map[0]);
-      tma_prefetch_desc(&p.map[1]);
       int it = 0, iv = 0;  // K and V tiles issued
       bool ok = true;
       while (ok && seg.next(p)) {
@@ -292,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         for (int i = 0; i < seg.n; ++i) {
           const int s = it % kStages;
           const uint32_t ph = ((it / kStages) & 1) ^ 1;
-          const int key0 = seg.lo + (seg.first + i) * kTile;
+          const int key0 = seg.cur_lo + (seg.first + i) * kTile;
           if (!(ok = mbar_wait(&k_empty[s], ph, abort_flag))) break;
           mbar_arrive_expect_tx(&k_full[s], kTileBytes);
           tma_load_3d(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row);
@@ -332,9 +360,9 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     };
     int it = 0, nseg = 0;
     while (ok && seg.next(p)) {
-      // the softmax warps write a segment's Q after they have taken the last O of the one before
-      while (ok && pv < it) ok = issue_pv();
-      ok = ok && warp_wait(q_full, nseg & 1, abort_flag);
+      // (a segment's Q is written once the last scores of the one before are there, so before that
+      // segment's last P)
+      ok = warp_wait(q_full, nseg & 1, abort_flag);
       ++nseg;
       for (int i = 0; i < seg.n && ok; ++i, ++it) {
         const int s = it % kStages;
@@ -361,85 +389,95 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     bool ok = true;
     int it = 0, nseg = 0;
     int64_t tile_id = share[4];  // of the whole batch
-    while (ok && seg.next(p)) {
+    // Q of a segment: 16 threads per head, 8 dims each
+    auto load_q = [&](const Segments& sg) {
+      const int h = tid >> 4, hb = sg.cur_u % p.nhb;
+      if (h >= min(kHeads, p.r - hb * kHeads)) return make_uint4(0, 0, 0, 0);
+      const int head = (sg.cur_u / p.nhb) * p.r + hb * kHeads + h;
+      return *reinterpret_cast<const uint4*>(p.q + sg.cur_b * p.q_sb + head * p.q_sh + 8 * (tid & 15));
+    };
+    // its parts into shared memory, once the scores of the segment before are done
+    auto write_q = [&](uint4 w, int parity) {
+      const int h = tid >> 4, c = tid & 15;
+      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+      float x[8];
+      float amax = 0.0f;
+      bool finite = true;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        x[i] = __uint_as_float((i & 1) ? (wd[i >> 1] & 0xFFFF0000u) : (wd[i >> 1] << 16));
+        finite = finite && fabsf(x[i]) < INFINITY;
+        amax = fmaxf(amax, fabsf(x[i]));
+      }
+#pragma unroll
+      for (int o = 1; o < 16; o <<= 1) {
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, o) != 0 && finite;
+      }
+      if (h < kHeads) {
+        uint32_t lo[kParts], hi[kParts];  // bytes of dims 0-3 and 4-7
+        float unit;                       // value of one step of the parts' sum
+        if constexpr (kInt8) {
+          unit = amax / kInt8One;
+          const float inv = (amax > 0.0f && finite) ? 1.0f / amax : 0.0f;
+#pragma unroll
+          for (int pt = 0; pt < kParts; ++pt) lo[pt] = hi[pt] = 0u;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const uint32_t v = split_int8(x[i] * inv);
+#pragma unroll
+            for (int pt = 0; pt < kParts; ++pt) {
+              const uint32_t byte = (v >> (16 - 8 * pt)) & 0xFFu;
+              if (i < 4) lo[pt] |= byte << (8 * i); else hi[pt] |= byte << (8 * (i - 4));
+            }
+          }
+        } else {
+          unit = amax > 0.0f ? pow2_at_least_448th(amax) : 1.0f;  // a power of two: x / unit is exact
+          const float inv = finite ? 1.0f / unit : 0.0f;
+          uint16_t pr[4][kParts];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) split_e4m3(__floats2half2_rn(x[2 * i] * inv, x[2 * i + 1] * inv), pr[i]);
+#pragma unroll
+          for (int pt = 0; pt < kParts; ++pt) {
+            lo[pt] = pr[0][pt] | (static_cast<uint32_t>(pr[1][pt]) << 16);
+            hi[pt] = pr[2][pt] | (static_cast<uint32_t>(pr[3][pt]) << 16);
+          }
+        }
+#pragma unroll
+        for (int pt = 0; pt < kParts; ++pt) {
+          const int n = pt * kHeads + h;
+          *reinterpret_cast<uint2*>(smem + Sm::q + n * 128 + (((c >> 1) ^ (n & 7)) << 4) + 8 * (c & 1)) =
+              make_uint2(lo[pt], hi[pt]);
+        }
+        // a query with an infinity or NaN has no finite score: NaN all through
+        if (c == 0) qf[8 * parity + h] = finite ? p.scale_log2 * unit : __uint_as_float(0x7FC00000u);
+      }
+      fence_proxy_async_smem();
+      mbar_arrive(q_full);
+    };
+    Segments ahead = seg;  // one segment further on, whose Q is loaded while this one runs
+    bool more = ahead.next(p);
+    if (more) write_q(load_q(ahead), 0);
+    while (ok && more) {
+      seg = ahead;
+      more = ahead.next(p);
+      const uint4 q_next = more ? load_q(ahead) : make_uint4(0, 0, 0, 0);
       const int g = seg.cur_u / p.nhb, hb = seg.cur_u % p.nhb;
       const int head0 = g * p.r + hb * kHeads;           // first query head of the block
       const int nh = min(kHeads, p.r - hb * kHeads);     // heads that exist
-      // Q parts: 16 threads per head, 8 dims each
-      {
-        const int h = tid >> 4, c = tid & 15;
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (h < nh)
-          w = *reinterpret_cast<const uint4*>(p.q + seg.cur_b * p.q_sb + (head0 + h) * p.q_sh + 8 * c);
-        const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-        float x[8];
-        float amax = 0.0f;
-        bool finite = true;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          x[i] = __uint_as_float((i & 1) ? (wd[i >> 1] & 0xFFFF0000u) : (wd[i >> 1] << 16));
-          finite = finite && fabsf(x[i]) < INFINITY;
-          amax = fmaxf(amax, fabsf(x[i]));
-        }
-#pragma unroll
-        for (int o = 1; o < 16; o <<= 1) {
-          amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-          finite = __shfl_xor_sync(0xffffffffu, finite ? 1 : 0, o) != 0 && finite;
-        }
-        if (h < kHeads) {
-          uint32_t lo[kParts], hi[kParts];  // bytes of dims 0-3 and 4-7
-          float unit;                       // value of one step of the parts' sum
-          if constexpr (kInt8) {
-            unit = amax / kInt8One;
-            const float inv = (amax > 0.0f && finite) ? 1.0f / amax : 0.0f;
-#pragma unroll
-            for (int pt = 0; pt < kParts; ++pt) lo[pt] = hi[pt] = 0u;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t v = split_int8(x[i] * inv);
-#pragma unroll
-              for (int pt = 0; pt < kParts; ++pt) {
-                const uint32_t byte = (v >> (16 - 8 * pt)) & 0xFFu;
-                if (i < 4) lo[pt] |= byte << (8 * i); else hi[pt] |= byte << (8 * (i - 4));
-              }
-            }
-          } else {
-            unit = amax > 0.0f ? pow2_at_least_448th(amax) : 1.0f;  // a power of two: x / unit is exact
-            const float inv = finite ? 1.0f / unit : 0.0f;
-            uint16_t pr[4][kParts];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) split_e4m3(__floats2half2_rn(x[2 * i] * inv, x[2 * i + 1] * inv), pr[i]);
-#pragma unroll
-            for (int pt = 0; pt < kParts; ++pt) {
-              lo[pt] = pr[0][pt] | (static_cast<uint32_t>(pr[1][pt]) << 16);
-              hi[pt] = pr[2][pt] | (static_cast<uint32_t>(pr[3][pt]) << 16);
-            }
-          }
-#pragma unroll
-          for (int pt = 0; pt < kParts; ++pt) {
-            const int n = pt * kHeads + h;
-            *reinterpret_cast<uint2*>(smem + Sm::q + n * 128 + (((c >> 1) ^ (n & 7)) << 4) + 8 * (c & 1)) =
-                make_uint2(lo[pt], hi[pt]);
-          }
-          // a query with an infinity or NaN has no finite score: NaN all through
-          if (c == 0) qf[h] = finite ? p.scale_log2 * unit : __uint_as_float(0x7FC00000u);
-        }
-        fence_proxy_async_smem();
-        mbar_arrive(q_full);
-      }
       if (!(ok = warp_wait(q_full, nseg & 1, abort_flag))) break;
       float f[kHeads], m[kHeads], l[kHeads], o[kHeads], alpha[kHeads], beta[kHeads];
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
-        f[h] = qf[h];
+        f[h] = qf[8 * (nseg & 1) + h];
         m[h] = -INFINITY;
         l[h] = o[h] = alpha[h] = beta[h] = 0.0f;
       }
       const int64_t kvrow = static_cast<int64_t>(seg.cur_b) * p.Hkv + g;
       const float* ks_row = p.scale[0] + kvrow * p.nblk;
       const float* vs_row = p.scale[1] + kvrow * p.nblk;
-      const int key_first = seg.lo + seg.first * kTile + tid;
-      int blk = min(key_first, seg.hi - 1) >> p.block_shift;
+      const int key_first = seg.cur_lo + seg.first * kTile + tid;
+      int blk = min(key_first, seg.cur_hi - 1) >> p.block_shift;
       float ks_next = ks_row[blk], vs_next = vs_row[blk];
       // adds O^T of tile t (relative to that tile's maximum and V scale)
       auto take_o = [&](int t) {
@@ -452,11 +490,11 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         return true;
       };
       for (int i = 0; i < seg.n && ok; ++i, ++it) {
-        const int key0 = seg.lo + (seg.first + i) * kTile;
-        const bool legal = key0 + tid < seg.hi;
+        const int key0 = seg.cur_lo + (seg.first + i) * kTile;
+        const bool legal = key0 + tid < seg.cur_hi;
         const float ks = ks_next, vs = legal ? vs_next : 0.0f;
         if (i + 1 < seg.n) {
-          blk = min(key0 + kTile + tid, seg.hi - 1) >> p.block_shift;
+          blk = min(key0 + kTile + tid, seg.cur_hi - 1) >> p.block_shift;
           ks_next = ks_row[blk];
           vs_next = vs_row[blk];
         }
@@ -470,6 +508,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) s[h] = legal ? join_parts<kInt8, kHeads>(c, h) * (f[h] * ks) : -INFINITY;
         }
+        if (more && i + 1 == seg.n) write_q(q_next, (nseg + 1) & 1);  // the last scores with this Q are done
         if constexpr (kWeights) {
           float* dst = p.scores + tile_id * kHeads * kTile + tid;
 #pragma unroll
@@ -533,7 +572,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
             }
           }
         }
-        if (key0 + kTile > seg.hi) {
+        if (key0 + kTile > seg.cur_hi) {
           // rows past the legal keys: whatever the cache holds there (a NaN byte, say) must not
           // meet P = 0 in the product
           const int st = it % kStages;
@@ -558,11 +597,21 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       if (!ok) break;
       // row sums over the keys (threads)
       float* lb = lred + (nseg & 1) * 32;
+      {
+        // over the warp, halving the heads with the first steps: lanes (32 / kHeads) h .. end with head h
+        int x = 16;
 #pragma unroll
-      for (int h = 0; h < kHeads; ++h) {
+        for (int k = kHeads / 2; k >= 1; k >>= 1, x >>= 1) {
+          const bool up = (lane & x) != 0;
 #pragma unroll
-        for (int x = 1; x < 32; x <<= 1) l[h] += __shfl_xor_sync(0xffffffffu, l[h], x);
-        if (lane == 0) lb[warp * 8 + h] = l[h];
+          for (int j = 0; j < k; ++j) {
+            const float give = up ? l[j] : l[j + k];
+            l[j] = (up ? l[j + k] : l[j]) + __shfl_xor_sync(0xffffffffu, give, x);
+          }
+        }
+#pragma unroll
+        for (; x >= 1; x >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
+        if (lane % (32 / kHeads) == 0) lb[warp * 8 + lane / (32 / kHeads)] = l[0];
       }
       __syncwarp();
       if (lane == 0) mbar_arrive(l_full);
@@ -573,7 +622,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         const float sum = (lb[h] + lb[8 + h]) + (lb[16 + h] + lb[24 + h]);
         if (tid == h) reinterpret_cast<float2*>(p.part_ml)[slot * kHeads + h] = make_float2(m[h], sum);
         if (h >= nh) continue;
-        if (seg.n == seg.all) {  // the whole unit: no merge
+        if (seg.n == seg.cur_all) {  // the whole unit: no merge
           const int64_t row = static_cast<int64_t>(seg.cur_b) * p.Hq + head0 + h;
           p.out[row * 128 + tid] = __float2bfloat16_rn(o[h] / sum);
           if (tid == h) p.lse[row] = lg2_approx(sum) + m[h];
@@ -631,17 +680,32 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
     const int nseg = last - first + 1;
     const int64_t slot0 = static_cast<int64_t>(sh.x) + first;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
-    float M = -INFINITY, L = 0.0f;
-    for (int i = lane; i < nseg; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * kHeads].x);
-    M = warp_max(M);
+    // 32 segments at a time, a lane each for their maxima and sums; their O rows are on the way meanwhile
     const float* po = p.part_o + (slot0 * kHeads + h) * 128 + tid;
-    float acc = 0.0f;
-#pragma unroll 8
-    for (int i = 0; i < nseg; ++i) {
-      const float2 x = ml[static_cast<int64_t>(i) * kHeads];
-      const float w = ex2_approx(x.x - M);
-      L = fmaf(x.y, w, L);
-      acc = fmaf(po[static_cast<int64_t>(i) * kHeads * 128], w, acc);
+    float M = -INFINITY, L = 0.0f, acc = 0.0f;
+    for (int i0 = 0; i0 < nseg; i0 += 32) {
+      const int cnt = min(32, nseg - i0);
+      const float2 x = lane < cnt ? ml[static_cast<int64_t>(i0 + lane) * kHeads] : make_float2(-INFINITY, 0.0f);
+      float v[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = j < cnt ? po[static_cast<int64_t>(i0 + j) * kHeads * 128] : 0.0f;
+      const float mn = fmaxf(M, warp_max(x.x));
+      const float w = lane < cnt ? ex2_approx(x.x - mn) : 0.0f;
+      const float scale = M == -INFINITY ? 0.0f : ex2_approx(M - mn);
+      float sum = x.y * w;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+      L = fmaf(L, scale, sum);
+      acc *= scale;
+      M = mn;
+      for (int j0 = 0; j0 < cnt; j0 += 8) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          acc = fmaf(v[j], __shfl_sync(0xffffffffu, w, j0 + j), acc);
+          const int k = j0 + 8 + j;
+          v[j] = k < cnt ? po[static_cast<int64_t>(i0 + k) * kHeads * 128] : 0.0f;
+        }
+      }
     }
     const int64_t row = static_cast<int64_t>(b) * p.Hq + (u / p.nhb) * p.r + hb * kHeads + h;
     p.out[row * 128 + tid] = __float2bfloat16_rn(acc / L);
@@ -655,6 +719,7 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
     seg.u = sh.x % units;
     seg.off = sh.y;
     seg.left = sh.z;
+    seg.sequence(p);
     int t = c * per;  // first tile of the segment, of the whole batch
     while (seg.next(p)) {
       const int g = seg.cur_u / p.nhb, hb0 = seg.cur_u % p.nhb;
@@ -662,8 +727,8 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
         float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
         for (int hb = 0; hb < p.nhb; ++hb) {
           const int nh = min(kHeads, p.r - hb * kHeads);
-          const int t0 = t - seg.first + hb * seg.all;  // first tile of the unit
-          const int first = t0 / per, last = (t0 + seg.all - 1) / per;
+          const int t0 = t - seg.first + hb * seg.cur_all;  // first tile of the unit
+          const int first = t0 / per, last = (t0 + seg.cur_all - 1) / per;
           const int64_t slot0 = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first;
           __syncthreads();
           if ((threadIdx.x & 96) == 0 && h < nh) {  // the head's lse from its segments
@@ -682,8 +747,8 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
           __syncthreads();
           const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + tid;
           for (int i = h + kHeads * (blockIdx.y - 1); i < seg.n; i += kHeads * (gridDim.y - 1)) {
-            const int key = seg.lo + (seg.first + i) * kTile + tid;
-            if (key >= seg.hi) continue;
+            const int key = seg.cur_lo + (seg.first + i) * kTile + tid;
+            if (key >= seg.cur_hi) continue;
             const float before = dst[key];
             float s[kHeads];
 #pragma unroll
@@ -712,10 +777,10 @@ cudaError_t launch_main(const KvDecodeParams& p, cudaStream_t stream) {
     if (e != cudaSuccess) return e;
     if (dev < 64) attr_set[dev] = true;
   }
-  kv_decode_kernel<kInt8, kHeads, kWeights><<<p.ctas, kThreads, KvSmem<kHeads>::bytes, stream>>>(p);
-  e = cudaGetLastError();
+  e = launch_dependent(kv_decode_kernel<kInt8, kHeads, kWeights>, dim3(p.ctas), dim3(kThreads), KvSmem<kHeads>::bytes, stream, p);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kv_decode_merge_kernel<kHeads, kWeights>, dim3(p.ctas, kWeights ? 2 : 1), dim3(128 * kHeads), stream, p);
+  return launch_dependent(kv_decode_merge_kernel<kHeads, kWeights>, dim3(p.ctas, kWeights ? 2 : 1), dim3(128 * kHeads), 0,
+                          stream, p);
 }
 
 template <bool kInt8>
