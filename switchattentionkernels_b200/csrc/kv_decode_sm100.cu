@@ -642,34 +642,42 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   if (tid == 0) p.cta_status[cta] = *abort_flag ? kStatusTimeout : 0;
 }
 
-// Second kernel, one block of 128 threads per head of a head block for each CTA of the
-// first.  blockIdx.y = 0: where CTA c's share begins inside a unit that the CTA before
-// began, the block merges that unit's segments; the blocks also write the rows of
-// sequences without a key.  blockIdx.y >= 1 (with weights): the attention weights
-// 2^(s - lse) of the keys of CTA c's tiles, summed over the group's heads in a fixed
-// order and added to the accumulated ones, kHeads tiles at a time.
+// Second kernel, blocks (c, y) for each CTA c of the first.
+// y < kHeads: where c's share begins inside a unit that the CTA before began, the block
+// merges the segments of that unit's head y; the blocks also write the rows of
+// sequences without a key.
+// y >= kHeads (with weights): the attention weights 2^(s - lse) of the keys of c's tiles,
+// summed over the group's heads in a fixed order and added to the accumulated ones.  A
+// warp takes a tile at a time, with all of its scores (4 keys a lane, kHeads heads) in
+// flight at once: the pass is a chain of L2 latencies (share, sums, scores) over little data.
+constexpr int kMergeThreads = 128;
+constexpr int kWeightBlocks = 8;  // blocks over a CTA's tiles
+
 template <int kHeads, bool kWeights>
-__global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
+__global__ void __launch_bounds__(kMergeThreads) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
   __shared__ float lse_sh[kHeads];
-  const int tid = threadIdx.x & 127, h = threadIdx.x >> 7, lane = threadIdx.x & 31;
-  const int c = blockIdx.x;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int c = blockIdx.x, y = blockIdx.y;
   const int units = p.Hkv * p.nhb;
   cudaGridDependencySynchronize();
   const int4 sh = p.share[c];
   const int per = p.share[0].z;  // tiles of every CTA but the last ones
-  if (blockIdx.y == 0) {
-    if (c == 0) {
+  if (!kWeights || y < kHeads) {
+    const int h = y;
+    if (c == 0 && h == 0) {
       int st = 0;
-      for (int i = threadIdx.x; i < p.ctas; i += 128 * kHeads) st |= p.cta_status[i];
+      for (int i = tid; i < p.ctas; i += kMergeThreads) st |= p.cta_status[i];
       st = __syncthreads_or(st);
-      if (threadIdx.x == 0) *p.status = st != 0 ? kStatusTimeout : 0;
+      if (tid == 0) *p.status = st != 0 ? kStatusTimeout : 0;
     }
     for (int b = c; b < p.B; b += p.ctas) {
       if (p.seq_lens[b] > 0) continue;
       // no key: 0 / 0 and log2 0, as the prefill writes a row without a legal key
-      for (int64_t i = threadIdx.x; i < static_cast<int64_t>(p.Hq) * 128; i += 128 * kHeads)
-        p.out[static_cast<int64_t>(b) * p.Hq * 128 + i] = __float2bfloat16_rn(__uint_as_float(0x7FC00000u));
-      for (int i = threadIdx.x; i < p.Hq; i += 128 * kHeads) p.lse[static_cast<int64_t>(b) * p.Hq + i] = -INFINITY;
+      for (int hq = h; hq < p.Hq; hq += kHeads) {
+        const int64_t row = static_cast<int64_t>(b) * p.Hq + hq;
+        p.out[row * 128 + tid] = __float2bfloat16_rn(__uint_as_float(0x7FC00000u));
+        if (tid == 0) p.lse[row] = -INFINITY;
+      }
     }
     // sh.y tiles of the unit lie before this CTA's: the CTA before began it if it holds them all
     if (sh.z == 0 || sh.y == 0 || sh.y > per) return;
@@ -721,6 +729,8 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
     seg.left = sh.z;
     seg.sequence(p);
     int t = c * per;  // first tile of the segment, of the whole batch
+    const int wi = (y - kHeads) * (kMergeThreads / 32) + warp;  // this warp among the share's
+    constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);
     while (seg.next(p)) {
       const int g = seg.cur_u / p.nhb, hb0 = seg.cur_u % p.nhb;
       if (hb0 == 0) {  // a key's tile of the first head block stands for its tiles of the others
@@ -730,33 +740,46 @@ __global__ void __launch_bounds__(128 * kHeads) kv_decode_merge_kernel(const __g
           const int t0 = t - seg.first + hb * seg.cur_all;  // first tile of the unit
           const int first = t0 / per, last = (t0 + seg.cur_all - 1) / per;
           const int64_t slot0 = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first;
-          __syncthreads();
-          if ((threadIdx.x & 96) == 0 && h < nh) {  // the head's lse from its segments
+          const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + lane;
+          float s[kHeads][4], old[4];
+          auto load = [&](int i) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const int key = seg.cur_lo + (seg.first + i) * kTile + 32 * j + lane;
+              old[j] = key < seg.cur_hi ? dst[key] : 0.0f;
+#pragma unroll
+              for (int h = 0; h < kHeads; ++h)
+                s[h][j] = h < nh ? sc[(static_cast<int64_t>(i) * kHeads + h) * kTile + 32 * j] : -INFINITY;
+            }
+          };
+          if (wi < seg.n) load(wi);
+          __syncthreads();  // the sums of the head block before are read no more
+          for (int h = warp; h < nh; h += kMergeThreads / 32) {  // the head's lse from its segments
             const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
             float M = -INFINITY, L = 0.0f;
-            for (int i = lane; i <= last - first; i += 32) M = fmaxf(M, ml[static_cast<int64_t>(i) * kHeads].x);
-            M = warp_max(M);
             for (int i = lane; i <= last - first; i += 32) {
               const float2 x = ml[static_cast<int64_t>(i) * kHeads];
-              L = fmaf(x.y, ex2_approx(x.x - M), L);
+              const float mn = fmaxf(M, x.x);
+              L = fmaf(x.y, ex2_approx(x.x - mn), M == -INFINITY ? 0.0f : L * ex2_approx(M - mn));
+              M = mn;
             }
+            const float top = warp_max(M);
+            L = M == -INFINITY && L == 0.0f ? 0.0f : L * ex2_approx(M - top);
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            if (lane == 0) lse_sh[h] = lg2_approx(L) + M;
+            if (lane == 0) lse_sh[h] = lg2_approx(L) + top;
           }
           __syncthreads();
-          const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + tid;
-          for (int i = h + kHeads * (blockIdx.y - 1); i < seg.n; i += kHeads * (gridDim.y - 1)) {
-            const int key = seg.cur_lo + (seg.first + i) * kTile + tid;
-            if (key >= seg.cur_hi) continue;
-            const float before = dst[key];
-            float s[kHeads];
+          for (int i = wi; i < seg.n; i += kStep) {
+            if (i != wi) load(i);
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j) s[j] = j < nh ? sc[(static_cast<int64_t>(i) * kHeads + j) * kTile] : 0.0f;
-            float w = 0.0f;
+            for (int j = 0; j < 4; ++j) {
+              float w = 0.0f;
 #pragma unroll
-            for (int j = 0; j < kHeads; ++j) w += j < nh ? ex2_approx(s[j] - lse_sh[j]) : 0.0f;
-            dst[key] = before + w;
+              for (int h = 0; h < kHeads; ++h) w += h < nh ? ex2_approx(s[h][j] - lse_sh[h]) : 0.0f;
+              const int key = seg.cur_lo + (seg.first + i) * kTile + 32 * j + lane;
+              if (key < seg.cur_hi) dst[key] = old[j] + w;
+            }
           }
         }
       }
@@ -779,8 +802,8 @@ cudaError_t launch_main(const KvDecodeParams& p, cudaStream_t stream) {
   }
   e = launch_dependent(kv_decode_kernel<kInt8, kHeads, kWeights>, dim3(p.ctas), dim3(kThreads), KvSmem<kHeads>::bytes, stream, p);
   if (e != cudaSuccess) return e;
-  return launch_dependent(kv_decode_merge_kernel<kHeads, kWeights>, dim3(p.ctas, kWeights ? 2 : 1), dim3(128 * kHeads), 0,
-                          stream, p);
+  return launch_dependent(kv_decode_merge_kernel<kHeads, kWeights>, dim3(p.ctas, kHeads + (kWeights ? kWeightBlocks : 0)),
+                          dim3(kMergeThreads), 0, stream, p);
 }
 
 template <bool kInt8>
