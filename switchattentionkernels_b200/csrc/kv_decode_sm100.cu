@@ -643,18 +643,18 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
 }
 
 // Second kernel, blocks (c, y) for each CTA c of the first.
-// y < kHeads: where c's share begins inside a unit that the CTA before began, the block
-// merges the segments of that unit's head y; the blocks also write the rows of
-// sequences without a key.
-// y >= kHeads (with weights): the attention weights 2^(s - lse) of the keys of c's tiles,
+// The last kHeads values of y: where c's share begins inside a unit that the CTA before
+// began, a block merges the segments of one of that unit's heads; the blocks also
+// write the rows of sequences without a key.
+// The y before those (with weights; they are dispatched first): the attention weights 2^(s - lse) of the keys of c's tiles,
 // summed over the group's heads in a fixed order and added to the accumulated ones.  A
 // warp takes a tile at a time, with all of its scores (4 keys a lane, kHeads heads) in
 // flight at once: the pass is a chain of L2 latencies (share, sums, scores) over little data.
 constexpr int kMergeThreads = 128;
-constexpr int kWeightBlocks = 8;  // blocks over a CTA's tiles
+constexpr int kWeightBlocks = 4;  // blocks over a CTA's tiles
 
 template <int kHeads, bool kWeights>
-__global__ void __launch_bounds__(kMergeThreads) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
+__global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
   __shared__ float lse_sh[kHeads];
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int c = blockIdx.x, y = blockIdx.y;
@@ -662,8 +662,9 @@ __global__ void __launch_bounds__(kMergeThreads) kv_decode_merge_kernel(const __
   cudaGridDependencySynchronize();
   const int4 sh = p.share[c];
   const int per = p.share[0].z;  // tiles of every CTA but the last ones
-  if (!kWeights || y < kHeads) {
-    const int h = y;
+  constexpr int kFirstMerge = kWeights ? kWeightBlocks : 0;
+  if (y >= kFirstMerge) {
+    const int h = y - kFirstMerge;
     if (c == 0 && h == 0) {
       int st = 0;
       for (int i = tid; i < p.ctas; i += kMergeThreads) st |= p.cta_status[i];
@@ -729,7 +730,7 @@ __global__ void __launch_bounds__(kMergeThreads) kv_decode_merge_kernel(const __
     seg.left = sh.z;
     seg.sequence(p);
     int t = c * per;  // first tile of the segment, of the whole batch
-    const int wi = (y - kHeads) * (kMergeThreads / 32) + warp;  // this warp among the share's
+    const int wi = y * (kMergeThreads / 32) + warp;  // this warp among the share's
     constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);
     while (seg.next(p)) {
       const int g = seg.cur_u / p.nhb, hb0 = seg.cur_u % p.nhb;
