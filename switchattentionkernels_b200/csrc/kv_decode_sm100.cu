@@ -36,6 +36,7 @@ constexpr int kTileBytes = kTile * 128;
 #define SWA_ST 2
 #endif
 constexpr int kStages = SWA_ST;                 // K tiles and V tiles in flight
+constexpr int kScaleRing = 8;              // tiles whose block scales are held
 constexpr int kThreads = 192;
 constexpr int kParts = 3;
 constexpr float kE4m3Step = 16.0f;         // weight of an e4m3 part against the next
@@ -51,8 +52,9 @@ struct KvSmem {
   static constexpr uint32_t red = p + 2 * cols * 128;              // [2][4 warps][12] floats
   static constexpr uint32_t lred = red + 2 * 4 * 12 * 4;           // [2][4 warps][8] floats
   static constexpr uint32_t qf = lred + 2 * 4 * 8 * 4;             // [2][8] floats
-  static constexpr uint32_t bars = qf + 64;
-  static constexpr uint32_t misc = bars + 24 * 8;                  // tmem holder, abort flag, start of the share
+  static constexpr uint32_t sc = qf + 64;                          // [kScaleRing][2][16] floats: K, V scales of a tile
+  static constexpr uint32_t bars = sc + kScaleRing * 128;
+  static constexpr uint32_t misc = bars + 32 * 8;                  // tmem holder, abort flag, start of the share
   static constexpr uint32_t total = misc + 64;
   static constexpr uint32_t bytes = total + 1024;
 };
@@ -211,7 +213,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   uint64_t* q_full = red_full + 2;       // Q parts of a segment
   uint64_t* l_full = q_full + 1;         // the four warps' row sums of a segment
   uint64_t* done = l_full + 1;
-  static_assert(4 * kStages + 4 * 2 + 3 <= 24, "barrier space");
+  uint64_t* sc_full = done + 1;          // [kScaleRing] block scales of a tile in shared memory
+  static_assert(4 * kStages + 4 * 2 + 3 + kScaleRing <= 32, "barrier space");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + Sm::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::misc + 4);
   int* share = reinterpret_cast<int*>(smem + Sm::misc + 8);  // see Segments::start; [4]: first tile of the batch's
@@ -236,6 +239,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     mbar_init(q_full, 128);
     mbar_init(l_full, 4);
     mbar_init(done, 1);
+    for (int i = 0; i < kScaleRing; ++i) mbar_init(&sc_full[i], 32);
     *abort_flag = 0;
     share[3] = 0;
     fence_barrier_init();
@@ -311,32 +315,48 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   seg.start(share);
 
   if (warp == 4) {
-    // ------------------------------------------------------------ TMA producer
-    if (lane == 0 && ntiles > 0) {
-      int it = 0, iv = 0;  // K and V tiles issued
-      bool ok = true;
-      while (ok && seg.next(p)) {
-        const int row = seg.cur_b * p.Hkv + seg.cur_u / p.nhb;
-        for (int i = 0; i < seg.n; ++i) {
-          const int s = it % kStages;
-          const uint32_t ph = ((it / kStages) & 1) ^ 1;
-          const int key0 = seg.cur_lo + (seg.first + i) * kTile;
-          if (!(ok = mbar_wait(&k_empty[s], ph, abort_flag))) break;
+    // ------------------------------------------------------------ producer
+    // Lane 0 issues the tiles; the warp copies the tile's block scales (at most 9 of K and 9 of V)
+    // along with K, so that they are there when the scores are: a softmax thread that loaded its
+    // key's scales itself, one tile ahead, waited some 800 cycles a tile for them behind the
+    // tiles that fill the memory queues.  Slot t % kScaleRing is free: k_empty of tile t - kStages
+    // says that the scores of that tile are done, so that P of the tile two before is written
+    // and the scales up to there are read.
+    static_assert(kScaleRing >= kStages + 2, "scale ring");
+    int it = 0, iv = 0;  // K and V tiles issued
+    bool ok = true;
+    while (ok && seg.next(p)) {
+      const int row = seg.cur_b * p.Hkv + seg.cur_u / p.nhb;
+      const float* scales = p.scale[lane >> 4] + static_cast<int64_t>(row) * p.nblk;
+      for (int i = 0; i < seg.n; ++i) {
+        const int s = it % kStages;
+        const uint32_t ph = ((it / kStages) & 1) ^ 1;
+        const int key0 = seg.cur_lo + (seg.first + i) * kTile;
+        if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
+        if (lane == 0) {
           mbar_arrive_expect_tx(&k_full[s], kTileBytes);
           tma_load_3d(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row);
-          ++it;
-          if (!(ok = mbar_wait(&v_empty[s], ph, abort_flag))) break;
+        }
+        const int blk = (key0 >> p.block_shift) + (lane & 15);
+        if (blk <= (min(key0 + kTile, seg.cur_hi) - 1) >> p.block_shift)
+          cp_async_4(smem_u32(smem + Sm::sc + (it % kScaleRing) * 128 + lane * 4), scales + blk);
+        cp_async_arrive(&sc_full[it % kScaleRing]);
+        ++it;
+        if (!(ok = warp_wait(&v_empty[s], ph, abort_flag))) break;
+        if (lane == 0) {
           mbar_arrive_expect_tx(&v_full[s], kTileBytes);
           tma_load_3d(smem + Sm::v + s * kTileBytes, &p.map[1], &v_full[s], 0, key0, row);
-          ++iv;
         }
+        ++iv;
       }
-      if (*abort_flag) {
-        // let the loads already issued land before the CTA's shared memory is released
-        volatile int dummy = 0;
-        for (int t = max(0, it - kStages); t < it; ++t) mbar_wait(&k_full[t % kStages], (t / kStages) & 1, &dummy);
-        for (int t = max(0, iv - kStages); t < iv; ++t) mbar_wait(&v_full[t % kStages], (t / kStages) & 1, &dummy);
-      }
+    }
+    cp_async_commit();
+    cp_async_wait<0>();
+    if (*abort_flag && lane == 0) {
+      // let the loads already issued land before the CTA's shared memory is released
+      volatile int dummy = 0;
+      for (int t = max(0, it - kStages); t < it; ++t) mbar_wait(&k_full[t % kStages], (t / kStages) & 1, &dummy);
+      for (int t = max(0, iv - kStages); t < iv; ++t) mbar_wait(&v_full[t % kStages], (t / kStages) & 1, &dummy);
     }
   } else if (warp == 5) {
     // ------------------------------------------------------------ MMA issuer
@@ -473,12 +493,6 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         m[h] = -INFINITY;
         l[h] = o[h] = alpha[h] = beta[h] = 0.0f;
       }
-      const int64_t kvrow = static_cast<int64_t>(seg.cur_b) * p.Hkv + g;
-      const float* ks_row = p.scale[0] + kvrow * p.nblk;
-      const float* vs_row = p.scale[1] + kvrow * p.nblk;
-      const int key_first = seg.cur_lo + seg.first * kTile + tid;
-      int blk = min(key_first, seg.cur_hi - 1) >> p.block_shift;
-      float ks_next = ks_row[blk], vs_next = vs_row[blk];
       // adds O^T of tile t (relative to that tile's maximum and V scale)
       auto take_o = [&](int t) {
         if (!warp_wait(&o_full[t & 1], (t >> 1) & 1, abort_flag)) return false;
@@ -492,13 +506,11 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       for (int i = 0; i < seg.n && ok; ++i, ++it) {
         const int key0 = seg.cur_lo + (seg.first + i) * kTile;
         const bool legal = key0 + tid < seg.cur_hi;
-        const float ks = ks_next, vs = legal ? vs_next : 0.0f;
-        if (i + 1 < seg.n) {
-          blk = min(key0 + kTile + tid, seg.cur_hi - 1) >> p.block_shift;
-          ks_next = ks_row[blk];
-          vs_next = vs_row[blk];
-        }
         const int buf = it & 1;
+        if (!(ok = warp_wait(&sc_full[it % kScaleRing], (it / kScaleRing) & 1, abort_flag))) break;
+        const float* sc = reinterpret_cast<const float*>(smem + Sm::sc + (it % kScaleRing) * 128) +
+                          ((min(key0 + tid, seg.cur_hi - 1) >> p.block_shift) - (key0 >> p.block_shift));
+        const float ks = sc[0], vs = legal ? sc[16] : 0.0f;
         if (!(ok = warp_wait(&s_full[buf], (it >> 1) & 1, abort_flag))) break;
         tc_fence_after();
         float s[kHeads];
