@@ -64,7 +64,7 @@ KvDecodePlan plan_decode(int B, int Smax, int Hq, int Hkv, bool weights, int nsm
   d.slots = units + d.ctas;
   auto up = [](size_t x) { return (x + 255) / 256 * 256; };
   d.share = 256;  // the status word first
-  d.cta_status = up(d.share + static_cast<size_t>(d.ctas) * 16);
+  d.cta_status = up(d.share + static_cast<size_t>(d.ctas) * sizeof(swa::KvShare));
   d.ml = up(d.cta_status + static_cast<size_t>(d.ctas) * 4);
   d.o = up(d.ml + static_cast<size_t>(d.slots) * d.heads * 8);
   d.scores = up(d.o + static_cast<size_t>(d.slots) * d.heads * 512);
@@ -162,7 +162,7 @@ int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const v
   rc = device_sms(&nsm);
   if (rc != SWA_OK) return rc;
   const KvDecodePlan d = plan_decode(B, Smax, Hq, Hkv, key_weights != nullptr, nsm);
-  if (d.tiles >= (int64_t(1) << 31) || static_cast<int64_t>(B) * Hq + d.ctas >= (int64_t(1) << 31))
+  if (d.tiles >= (int64_t(1) << 28) || static_cast<int64_t>(B) * Hq + d.ctas >= (int64_t(1) << 31))
     return fail(SWA_E_UNSUPPORTED, "KV cache too large for 32-bit tile indices");
   if (workspace_bytes < d.bytes) return fail(SWA_E_INVALID, "workspace too small");
   swa::KvDecodeParams p{};
@@ -183,7 +183,7 @@ int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const v
   p.weights = key_weights;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   p.status = reinterpret_cast<int32_t*>(ws);
-  p.share = reinterpret_cast<int4*>(ws + d.share);
+  p.share = reinterpret_cast<swa::KvShare*>(ws + d.share);
   p.cta_status = reinterpret_cast<int32_t*>(ws + d.cta_status);
   p.part_ml = reinterpret_cast<float*>(ws + d.ml);
   p.part_o = reinterpret_cast<float*>(ws + d.o);

@@ -63,11 +63,24 @@ struct KvEvictParams {
 cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream);
 
 // Decode over the cache.  The (sequence, KV head, head block) units' legal keys are
-// cut into tiles of 128 keys, all tiles of the batch are laid end to end in the order
-// (sequence, KV head, head block, tile), and each of the `ctas` CTAs takes `per` =
-// ceil(tiles / ctas) consecutive ones.  A CTA's share of one unit is a segment; its
-// partial result lies in slot unit + cta (both grow along the order and each new
-// segment moves one of them, so slots are distinct).
+// cut into tiles of 128 keys.  All units of the batch are laid end to end along one axis
+// of work, in the order (sequence, KV head, head block), each as `omega` steps for
+// starting it and kTileSteps for every tile, and the axis is cut into equal shares, one
+// a CTA: a tile belongs to the CTA on whose share its first step lies.  A CTA's part of
+// one unit is a segment; its partial result lies in slot unit + cta (both grow along the
+// axis and each new segment moves one of them, so slots are distinct).
+constexpr int kTileSteps = 2;
+
+// What CTA c's share begins with, and the whole plan.
+struct __align__(16) KvShare {
+  int b, u, off, left;    // sequence, unit in it, first step in the unit, steps of the share
+  int vbase, tbase;       // steps and tiles of the batch before the unit
+  int lo, hi;             // legal keys of the sequence
+  int omega;              // of the batch, as are
+  int per, longer;        // steps of a share; the first `longer` shares have one more
+  int pad;
+};
+
 struct __align__(64) KvDecodeParams {
   CUtensorMap map[2];         // K, V bytes: 3-D {128, Smax, B * Hkv}, box {128, 128, 1}, 128B swizzle
   const __nv_bfloat16* q;     // element (b, h, d) at b * q_sb + h * q_sh + d
@@ -79,7 +92,7 @@ struct __align__(64) KvDecodeParams {
   float* lse;                 // [B, Hq]
   float* weights;             // [B, Hkv, Smax] added to, or null
   // workspace
-  int4* share;                // [ctas] {unit of the first tile, that tile's index in it, tiles, tiles of the unit}
+  KvShare* share;             // [ctas]
   int32_t* cta_status;        // [ctas]
   int32_t* status;
   float* part_ml;             // [slots, heads, 2] maximum and sum of each partial row
@@ -93,9 +106,6 @@ struct __align__(64) KvDecodeParams {
 };
 cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream);
 // Resident CTAs of the decode kernel per SM (what its shared memory allows).
-#ifndef SWA_CPS
-#define SWA_CPS 2
-#endif
-constexpr int kKvDecodeCtasPerSm = SWA_CPS;
+constexpr int kKvDecodeCtasPerSm = 2;
 
 }  // namespace swa

@@ -32,10 +32,7 @@ namespace {
 
 constexpr int kTile = 128;                 // keys of a tile
 constexpr int kTileBytes = kTile * 128;
-#ifndef SWA_ST
-#define SWA_ST 2
-#endif
-constexpr int kStages = SWA_ST;                 // K tiles and V tiles in flight
+constexpr int kStages = 2;                 // K tiles and V tiles in flight
 constexpr int kScaleRing = 8;              // tiles whose block scales are held
 constexpr int kThreads = 192;
 constexpr int kParts = 3;
@@ -54,8 +51,8 @@ struct KvSmem {
   static constexpr uint32_t qf = lred + 2 * 4 * 8 * 4;             // [2][8] floats
   static constexpr uint32_t sc = qf + 64;                          // [kScaleRing][2][16] floats: K, V scales of a tile
   static constexpr uint32_t bars = sc + kScaleRing * 128;
-  static constexpr uint32_t misc = bars + 32 * 8;                  // tmem holder, abort flag, start of the share
-  static constexpr uint32_t total = misc + 64;
+  static constexpr uint32_t misc = bars + 32 * 8;                  // tmem holder, abort flag, the share
+  static constexpr uint32_t total = misc + 16 + 64;
   static constexpr uint32_t bytes = total + 1024;
 };
 
@@ -81,53 +78,74 @@ __device__ __forceinline__ int seq_tiles(const KvDecodeParams& p, int b) {
   return (r.hi - r.lo + kTile - 1) / kTile;
 }
 
-// A CTA's share of the tiles, segment by segment.
-struct Segments {
-  int b, u, off, left;  // of the next segment: sequence, unit in it (KV head x head block), first tile; tiles left
-  int lo, hi, all;      // legal keys of sequence b, tiles of its units
-  // the current segment
-  int cur_b, cur_u, cur_lo, cur_hi, cur_all, first, n;
+// First step of share c of the axis of work, and the share that step v lies on.
+__device__ __forceinline__ int share_start(int c, int per, int longer) { return c * per + min(c, longer); }
+__device__ __forceinline__ int share_of(int v, int per, int longer) {
+  const int w = v - longer * (per + 1);
+  return w < 0 ? v / (per + 1) : longer + w / per;
+}
 
-  // share: {sequence, unit, tile, tiles, -, lo, hi, tiles of the unit}
-  __device__ __forceinline__ void start(const int* share) {
-    b = share[0];
-    u = share[1];
-    off = share[2];
-    left = share[3];
-    lo = share[5];
-    hi = share[6];
-    all = share[7];
+// Steps for starting a unit (its Q, its first tile's latency, the sums and the output at
+// its end), in half tiles.  On 64 sequences a CTA with six segments took 1.5 us more
+// per segment than one with a single one, at 1.2 us a tile: without these steps the CTAs of the
+// short units ended 8 us of 62 after the others.  With few tiles a CTA they do not
+// matter and every CTA takes whole tiles only.
+constexpr int kUnitSteps = 3;
+constexpr int kFewTiles = 4;
+
+// A CTA's share, segment by segment.
+struct Segments {
+  int b, u, off, left;  // of the next segment: sequence, unit in it (KV head x head block), first step in it; steps left
+  int vbase, tbase;     // steps and tiles of the batch before that unit
+  int lo, hi, all;      // legal keys of sequence b, tiles of its units
+  int omega;
+  // the current segment
+  int cur_b, cur_u, cur_vbase, cur_tbase, cur_lo, cur_hi, cur_all, first, n;
+
+  __device__ __forceinline__ void start(const KvShare& s) {
+    b = s.b;
+    u = s.u;
+    off = s.off;
+    left = s.left;
+    vbase = s.vbase;
+    tbase = s.tbase;
+    lo = s.lo;
+    hi = s.hi;
+    all = (hi - lo + kTile - 1) / kTile;
+    omega = s.omega;
   }
-  __device__ __forceinline__ void sequence(const KvDecodeParams& p) {
-    const KeyRange r = key_range(p, b);
-    lo = r.lo;
-    hi = r.hi;
-    all = (r.hi - r.lo + kTile - 1) / kTile;
-  }
+  // the next segment with a tile of this share; false when there is none
   __device__ __forceinline__ bool next(const KvDecodeParams& p) {
-    if (left <= 0) return false;
-    while (all == 0) {  // sequences without a key
-      ++b;
-      sequence(p);
-    }
-    cur_b = b;
-    cur_u = u;
-    cur_lo = lo;
-    cur_hi = hi;
-    cur_all = all;
-    first = off;
-    n = min(all - off, left);
-    left -= n;
-    off += n;
-    if (off == all) {
-      off = 0;
-      if (++u == p.Hkv * p.nhb) {
-        u = 0;
-        ++b;
-        if (left > 0) sequence(p);
+    while (left > 0) {
+      const int length = all > 0 ? omega + all * kTileSteps : 0;
+      const int take = min(length - off, left);
+      cur_b = b;
+      cur_u = u;
+      cur_vbase = vbase;
+      cur_tbase = tbase;
+      cur_lo = lo;
+      cur_hi = hi;
+      cur_all = all;
+      first = max(0, off - omega + kTileSteps - 1) / kTileSteps;
+      n = max(0, off + take - omega + kTileSteps - 1) / kTileSteps - first;
+      left -= take;
+      off += take;
+      if (off == length && left > 0) {
+        off = 0;
+        vbase += length;
+        tbase += all;
+        if (all == 0 || ++u == p.Hkv * p.nhb) {  // (a sequence without a key has no unit)
+          u = 0;
+          ++b;
+          const KeyRange r = key_range(p, b);
+          lo = r.lo;
+          hi = r.hi;
+          all = (r.hi - r.lo + kTile - 1) / kTile;
+        }
       }
+      if (n > 0) return true;
     }
-    return true;
+    return false;
   }
 };
 
@@ -217,7 +235,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   static_assert(4 * kStages + 4 * 2 + 3 + kScaleRing <= 32, "barrier space");
   uint32_t* tmem_holder = reinterpret_cast<uint32_t*>(smem + Sm::misc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Sm::misc + 4);
-  int* share = reinterpret_cast<int*>(smem + Sm::misc + 8);  // see Segments::start; [4]: first tile of the batch's
+  KvShare* share = reinterpret_cast<KvShare*>(smem + Sm::misc + 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
   const int units = p.Hkv * p.nhb;  // units of a sequence
@@ -241,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     mbar_init(done, 1);
     for (int i = 0; i < kScaleRing; ++i) mbar_init(&sc_full[i], 32);
     *abort_flag = 0;
-    share[3] = 0;
+    share->left = 0;
     fence_barrier_init();
   }
   if (tid == 128) {
@@ -262,57 +280,78 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     tmem_relinquish();
   }
   {
-    // this CTA's share: thread t sums the tiles of a run of sequences, then a scan over the threads
-    int* scan = reinterpret_cast<int*>(smem + Sm::red);
+    // this CTA's share: thread t sums a run of sequences' tiles and counts those that have any, then
+    // a scan of both (packed into 64 bits) over the threads
+    int64_t* scan = reinterpret_cast<int64_t*>(smem + Sm::red);
+    constexpr int64_t kOne = int64_t{1} << 32;
     const int run = (p.B + kThreads - 1) / kThreads;
     const int b0 = min(p.B, tid * run), b1 = min(p.B, b0 + run);
-    int sum = 0;
-    for (int b = b0; b < b1; ++b) sum += seq_tiles(p, b);
-    int incl = sum;
+    int64_t sum = 0;
+    for (int b = b0; b < b1; ++b) {
+      const int n = seq_tiles(p, b);
+      sum += n > 0 ? kOne + n : 0;
+    }
+    int64_t incl = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const int t = __shfl_up_sync(0xffffffffu, incl, o);
+      const int64_t t = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += t;
     }
     if (lane == 31) scan[warp] = incl;
     __syncthreads();
-    int before = incl - sum, total = 0;
+    int64_t before = incl - sum, total = 0;
     for (int w = 0; w < kThreads / 32; ++w) {
       if (w < warp) before += scan[w];
       total += scan[w];
     }
-    const int tiles = total * units;
-    const int per = (tiles + p.ctas - 1) / p.ctas;
-    const int t0 = cta * per, t1 = min(tiles, t0 + per);
-    if (t0 >= t1) {
-      if (tid == 0) p.share[cta] = make_int4(0, 0, 0, 0);
-    } else if (t0 >= before * units && t0 < (before + sum) * units) {  // exactly one thread
-      int b = b0, c = before * units;
-      for (;; ++b) {
-        const int nb = seq_tiles(p, b) * units;
-        if (t0 < c + nb) break;
-        c += nb;
+    const int tiles = static_cast<int>(total & (kOne - 1)) * units;
+    const int omega = tiles >= kFewTiles * p.ctas ? kUnitSteps : 0;
+    auto steps_of = [&](int64_t x) {  // of x's sequences and tiles
+      return (static_cast<int>(x >> 32) * omega + static_cast<int>(x & (kOne - 1)) * kTileSteps) * units;
+    };
+    const int steps = steps_of(total);
+    // every share holds the first step of a tile: they lie at most omega + kTileSteps apart
+    const int ctas = max(1, min(p.ctas, steps / (omega + kTileSteps)));
+    KvShare sh{};
+    sh.omega = omega;
+    sh.per = steps / ctas;
+    sh.longer = steps % ctas;
+    const int v0 = share_start(cta, sh.per, sh.longer), v1 = share_start(cta + 1, sh.per, sh.longer);
+    if (cta >= ctas || v0 >= v1) {
+      if (tid == 0) {
+        p.share[cta] = sh;
+        *share = sh;
       }
-      const int nb = seq_tiles(p, b);
-      share[0] = b;
-      share[1] = (t0 - c) / nb;
-      share[2] = (t0 - c) % nb;
-      share[3] = t1 - t0;
-      share[4] = t0;
-      const KeyRange kr = key_range(p, b);
-      share[5] = kr.lo;
-      share[6] = kr.hi;
-      share[7] = nb;
-      p.share[cta] = make_int4(b * units + share[1], share[2], t1 - t0, nb);
+    } else if (v0 >= steps_of(before) && v0 < steps_of(before + sum)) {  // exactly one thread
+      int64_t at = before;
+      for (int b = b0;; ++b) {
+        const int n = seq_tiles(p, b);
+        const int64_t next = at + (n > 0 ? kOne + n : 0);
+        if (v0 < steps_of(next)) {
+          const KeyRange kr = key_range(p, b);
+          const int length = omega + n * kTileSteps, in = v0 - steps_of(at);
+          sh.b = b;
+          sh.u = in / length;
+          sh.off = in % length;
+          sh.left = v1 - v0;
+          sh.vbase = v0 - sh.off;
+          sh.tbase = static_cast<int>(at & (kOne - 1)) * units + sh.u * n;
+          sh.lo = kr.lo;
+          sh.hi = kr.hi;
+          break;
+        }
+        at = next;
+      }
+      p.share[cta] = sh;
+      *share = sh;
     }
   }
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_holder;  // S: columns 0 and kCols, O: 2 kCols and 3 kCols
-  const int ntiles = share[3];
   Segments seg{};
-  seg.start(share);
+  seg.start(*share);
 
   if (warp == 4) {
     // ------------------------------------------------------------ producer
@@ -408,7 +447,6 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     float* qf = reinterpret_cast<float*>(smem + Sm::qf);
     bool ok = true;
     int it = 0, nseg = 0;
-    int64_t tile_id = share[4];  // of the whole batch
     // Q of a segment: 16 threads per head, 8 dims each
     auto load_q = [&](const Segments& sg) {
       const int h = tid >> 4, hb = sg.cur_u % p.nhb;
@@ -522,10 +560,9 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         }
         if (more && i + 1 == seg.n) write_q(q_next, (nseg + 1) & 1);  // the last scores with this Q are done
         if constexpr (kWeights) {
-          float* dst = p.scores + tile_id * kHeads * kTile + tid;
+          float* dst = p.scores + static_cast<int64_t>(seg.cur_tbase + seg.first + i) * kHeads * kTile + tid;
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) dst[h * kTile] = s[h];
-          ++tile_id;
         }
         // maxima of the tile over its keys
         float* rb = red + buf * 48;
@@ -655,8 +692,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
 }
 
 // Second kernel, blocks (c, y) for each CTA c of the first.
-// The last kHeads values of y: where c's share begins inside a unit that the CTA before
-// began, a block merges the segments of one of that unit's heads; the blocks also
+// The last kHeads values of y: where c's share holds the last but not the first tile of a
+// unit, a block merges the segments of one of that unit's heads; the blocks also
 // write the rows of sequences without a key.
 // The y before those (with weights; they are dispatched first): the attention weights 2^(s - lse) of the keys of c's tiles,
 // summed over the group's heads in a fixed order and added to the accumulated ones.  A
@@ -672,8 +709,9 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
   const int c = blockIdx.x, y = blockIdx.y;
   const int units = p.Hkv * p.nhb;
   cudaGridDependencySynchronize();
-  const int4 sh = p.share[c];
-  const int per = p.share[0].z;  // tiles of every CTA but the last ones
+  const KvShare sh = p.share[c];
+  Segments seg{};
+  seg.start(sh);
   constexpr int kFirstMerge = kWeights ? kWeightBlocks : 0;
   if (y >= kFirstMerge) {
     const int h = y - kFirstMerge;
@@ -692,14 +730,13 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
         if (tid == 0) p.lse[row] = -INFINITY;
       }
     }
-    // sh.y tiles of the unit lie before this CTA's: the CTA before began it if it holds them all
-    if (sh.z == 0 || sh.y == 0 || sh.y > per) return;
-    const int b = sh.x / units, u = sh.x % units;
+    if (!seg.next(p) || seg.first == 0 || seg.first + seg.n < seg.cur_all) return;
+    const int b = seg.cur_b, u = seg.cur_u;
     const int hb = u % p.nhb;
     if (h >= min(kHeads, p.r - hb * kHeads)) return;
-    const int first = c - 1, last = (c * per - sh.y + sh.w - 1) / per;
-    const int nseg = last - first + 1;
-    const int64_t slot0 = static_cast<int64_t>(sh.x) + first;
+    const int first = share_of(seg.cur_vbase + sh.omega, sh.per, sh.longer);
+    const int nseg = c - first + 1;
+    const int64_t slot0 = static_cast<int64_t>(b) * units + u + first;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
     // 32 segments at a time, a lane each for their maxima and sums; their O rows are on the way meanwhile
     const float* po = p.part_o + (slot0 * kHeads + h) * 128 + tid;
@@ -734,14 +771,6 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
     return;
   }
   if constexpr (kWeights) {
-    if (sh.z == 0) return;
-    Segments seg{};
-    seg.b = sh.x / units;
-    seg.u = sh.x % units;
-    seg.off = sh.y;
-    seg.left = sh.z;
-    seg.sequence(p);
-    int t = c * per;  // first tile of the segment, of the whole batch
     const int wi = y * (kMergeThreads / 32) + warp;  // this warp among the share's
     constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);
     while (seg.next(p)) {
@@ -750,8 +779,10 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
         float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
         for (int hb = 0; hb < p.nhb; ++hb) {
           const int nh = min(kHeads, p.r - hb * kHeads);
-          const int t0 = t - seg.first + hb * seg.cur_all;  // first tile of the unit
-          const int first = t0 / per, last = (t0 + seg.cur_all - 1) / per;
+          const int t0 = seg.cur_tbase + hb * seg.cur_all;  // first tile of the unit
+          const int v0 = seg.cur_vbase + sh.omega + hb * (sh.omega + seg.cur_all * kTileSteps);  // and its first step
+          const int first = share_of(v0, sh.per, sh.longer);
+          const int last = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer);
           const int64_t slot0 = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first;
           const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + lane;
           float s[kHeads][4], old[4];
@@ -796,7 +827,6 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
           }
         }
       }
-      t += seg.n;
     }
   }
 }
