@@ -176,8 +176,9 @@ template <bool kInt8, int kPasses>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
   constexpr int kBlock = 16 * kPasses;
   const int b = blockIdx.z, g = blockIdx.y >> 1, kv = blockIdx.y & 1;
-  const RowRange rg = append_range(p, b);
+  cudaGridDependencySynchronize();
   cudaTriggerProgrammaticLaunchCompletion();
+  const RowRange rg = append_range(p, b);
   if (!p.lens_after && blockIdx.x == 0 && blockIdx.y == 0 && threadIdx.x == 0) p.seq_lens[b] = rg.end;
   const int blk = rg.start / kBlock + blockIdx.x;
   const int row0 = blk * kBlock;
@@ -242,6 +243,7 @@ __global__ void kv_advance_kernel(const __grid_constant__ KvAppendParams p) {
 template <bool kInt8>
 __global__ void __launch_bounds__(1024) kv_append_token_kernel(const __grid_constant__ KvAppendParams p) {
   const int b = blockIdx.x, lane = threadIdx.x & 31;
+  cudaGridDependencySynchronize();
   const RowRange rg = append_range(p, b);
   if (rg.end > rg.start) {
     const int blk = rg.start / p.block, row0 = blk * p.block;
@@ -278,16 +280,13 @@ __global__ void __launch_bounds__(1024) kv_append_token_kernel(const __grid_cons
 
 template <bool kInt8>
 cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
+  void (*kernel)(KvAppendParams) = p.block == 16   ? kv_append_kernel<kInt8, 1>
+                                   : p.block == 32 ? kv_append_kernel<kInt8, 2>
+                                   : p.block == 64 ? kv_append_kernel<kInt8, 4>
+                                                   : kv_append_kernel<kInt8, 8>;
   const dim3 grid((p.T - 1) / p.block + 2, 2 * p.Hkv, p.B);
-  switch (p.block) {
-    case 16: kv_append_kernel<kInt8, 1><<<grid, kAppendThreads, 0, stream>>>(p); break;
-    case 32: kv_append_kernel<kInt8, 2><<<grid, kAppendThreads, 0, stream>>>(p); break;
-    case 64: kv_append_kernel<kInt8, 4><<<grid, kAppendThreads, 0, stream>>>(p); break;
-    default: kv_append_kernel<kInt8, 8><<<grid, kAppendThreads, 0, stream>>>(p); break;
-  }
-  cudaError_t e = cudaGetLastError();
-  if (e != cudaSuccess) return e;
-  if (!p.lens_after) return cudaSuccess;
+  cudaError_t e = launch_dependent(kernel, grid, dim3(kAppendThreads), 0, stream, p);
+  if (e != cudaSuccess || !p.lens_after) return e;
   return launch_dependent(kv_advance_kernel, dim3((p.B + 127) / 128), dim3(128), 0, stream, p);
 }
 
@@ -328,6 +327,8 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   const int64_t unit = blockIdx.x / ncta;
   const int b = static_cast<int>(unit / p.Hkv);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  cudaGridDependencySynchronize();
+  cudaTriggerProgrammaticLaunchCompletion();
   const int L = min(max(p.seq_lens[b], 0), p.Smax);
   int32_t* slots = p.slots + unit * p.n;
   if (L <= p.keep) {  // nothing to evict (the whole cluster agrees)
@@ -449,30 +450,15 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   });
 }
 
-template <int kPerThread>
-cudaError_t launch_select(const KvEvictParams& p, int cluster, cudaStream_t stream) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(p.B * p.Hkv * cluster);
-  cfg.blockDim = dim3(kSelThreads);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = cluster;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  return cudaLaunchKernelEx(&cfg, kv_select_kernel<kPerThread>, p);
-}
-
 // CTAs per (sequence, KV head): 8 weights a thread, as few CTAs as hold a sequence of
 // the largest length; above 8 CTAs' 65536 rows 16 a thread, above 131072 none are held.
 cudaError_t launch_select(const KvEvictParams& p, cudaStream_t stream) {
   int cluster = 1;
   while (cluster < kSelMaxCluster && p.Smax > cluster * kSelThreads * 8) cluster *= 2;
-  if (p.Smax <= cluster * kSelThreads * 8) return launch_select<8>(p, cluster, stream);
-  if (p.Smax <= cluster * kSelThreads * 16) return launch_select<16>(p, cluster, stream);
-  return launch_select<0>(p, cluster, stream);
+  void (*kernel)(KvEvictParams) = p.Smax <= cluster * kSelThreads * 8    ? kv_select_kernel<8>
+                                  : p.Smax <= cluster * kSelThreads * 16 ? kv_select_kernel<16>
+                                                                         : kv_select_kernel<0>;
+  return launch_cluster_dependent(cluster, kernel, dim3(p.B * p.Hkv * cluster), dim3(kSelThreads), 0, stream, p);
 }
 
 // ---------------------------------------------------------------------------
@@ -587,15 +573,17 @@ template <bool kInt8>
 __global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ KvEvictParams p, int tiles) {
   const int64_t unit = blockIdx.x / tiles;
   const int tile = blockIdx.x % tiles;
+  cudaGridDependencySynchronize();
   move_rows<kInt8, false>(p, unit, tile * kMoveRows, false);
   if (tile == 0) write_kept_length(p, unit);
 }
 
 template <bool kInt8>
-__global__ void __cluster_dims__(kMoveCluster, 1, 1) __launch_bounds__(kMoveThreads)
+__global__ void __launch_bounds__(kMoveThreads)
     kv_move_in_place_kernel(const __grid_constant__ KvEvictParams p) {
   const int64_t unit = blockIdx.x / kMoveCluster;
   const int rank = blockIdx.x % kMoveCluster;
+  cudaGridDependencySynchronize();
   for (int step = 0; step < p.n; step += kMoveCluster * kMoveRows) {
     move_rows<kInt8, true>(p, unit, step + rank * kMoveRows, true);
     __syncthreads();
@@ -606,37 +594,22 @@ __global__ void __cluster_dims__(kMoveCluster, 1, 1) __launch_bounds__(kMoveThre
 }  // namespace
 
 cudaError_t launch_kv_append(const KvAppendParams& p, bool int8, cudaStream_t stream) {
-  if (p.T == 1) {
-    const int threads = 32 * (2 * p.Hkv < 32 ? 2 * p.Hkv : 32);
-    if (int8) {
-      kv_append_token_kernel<true><<<p.B, threads, 0, stream>>>(p);
-    } else {
-      kv_append_token_kernel<false><<<p.B, threads, 0, stream>>>(p);
-    }
-    return cudaGetLastError();
-  }
-  return int8 ? append_rows<true>(p, stream) : append_rows<false>(p, stream);
+  if (p.T > 1) return int8 ? append_rows<true>(p, stream) : append_rows<false>(p, stream);
+  const int threads = 32 * (2 * p.Hkv < 32 ? 2 * p.Hkv : 32);
+  return launch_dependent(int8 ? kv_append_token_kernel<true> : kv_append_token_kernel<false>, dim3(p.B), dim3(threads), 0,
+                          stream, p);
 }
 
 cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream) {
-  const int units = p.B * p.Hkv;
   cudaError_t e = launch_select(p, stream);
   if (e != cudaSuccess) return e;
-  if (in_place) {
-    if (int8) {
-      kv_move_in_place_kernel<true><<<units * kMoveCluster, kMoveThreads, 0, stream>>>(p);
-    } else {
-      kv_move_in_place_kernel<false><<<units * kMoveCluster, kMoveThreads, 0, stream>>>(p);
-    }
-  } else {
-    const int tiles = (p.n + kMoveRows - 1) / kMoveRows;
-    if (int8) {
-      kv_move_kernel<true><<<units * tiles, kMoveThreads, 0, stream>>>(p, tiles);
-    } else {
-      kv_move_kernel<false><<<units * tiles, kMoveThreads, 0, stream>>>(p, tiles);
-    }
-  }
-  return cudaGetLastError();
+  const int units = p.B * p.Hkv;
+  if (in_place)
+    return launch_cluster_dependent(kMoveCluster, int8 ? kv_move_in_place_kernel<true> : kv_move_in_place_kernel<false>,
+                                    dim3(units * kMoveCluster), dim3(kMoveThreads), 0, stream, p);
+  const int tiles = (p.n + kMoveRows - 1) / kMoveRows;
+  return launch_dependent(int8 ? kv_move_kernel<true> : kv_move_kernel<false>, dim3(units * tiles), dim3(kMoveThreads), 0,
+                          stream, p, tiles);
 }
 
 }  // namespace swa
