@@ -142,7 +142,8 @@ def _on(dev: torch.device):
 
 
 def _stream(dev: torch.device) -> int:
-    return torch.cuda.current_stream(dev).cuda_stream
+    """The current stream's handle (without the Stream object that ``torch.cuda.current_stream`` makes)."""
+    return torch._C._cuda_getCurrentRawStream(dev.index)
 
 
 @lru_cache(maxsize=256)
@@ -234,11 +235,11 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
         raise ValueError("sm_scale must be positive")
     _core._check_status_out(status_out, dev)
     weights = cache.key_weights if accumulate else None
-    out = torch.empty((B, Hq, HEAD_DIM), dtype=torch.bfloat16, device=dev)
-    lse = torch.empty((B, Hq), dtype=torch.float32, device=dev)
+    out = q.new_empty((B, Hq, HEAD_DIM))
+    lse = cache.k_scale.new_empty((B, Hq))
     with _on(dev):
         nbytes = _decode_workspace_bytes(B, Smax, Hq, Hkv, weights is not None, dev.index)
-        ws = torch.empty((nbytes + 15) // 16 * 4, dtype=torch.int32, device=dev)
+        ws = cache.seq_lens.new_empty((nbytes + 15) // 16 * 4)
         route = route_full if route_full.is_contiguous() else route_full.contiguous()
         rc = _native.load().swa_kv_decode(
             q.data_ptr(), st[0], st[1], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
@@ -295,7 +296,7 @@ def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, rec
             if first < ends[1 - owner]:
                 raise ValueError("out must not share memory with the cache")
             ends[owner] = max(ends[owner], end)
-    slots = torch.empty((B, Hkv, keep), dtype=torch.int32, device=dev)
+    slots = cache.seq_lens.new_empty((B, Hkv, keep))
     with _on(dev):
         rc = _native.load().swa_kv_evict(*src, *dst, slots.data_ptr(), B, Hkv, Smax, So, HEAD_DIM, cache.block_size,
                                          keep, sink, recent, _DTYPES[cache.k.dtype], _stream(dev))
