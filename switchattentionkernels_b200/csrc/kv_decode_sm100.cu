@@ -362,6 +362,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     // says that the scores of that tile are done, so that P of the tile two before is written
     // and the scales up to there are read.
     static_assert(kScaleRing >= kStages + 2, "scale ring");
+    const uint64_t once = l2_policy_evict_first();
     int it = 0, iv = 0;  // K and V tiles issued
     bool ok = true;
     while (ok && seg.next(p)) {
@@ -374,7 +375,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&k_full[s], kTileBytes);
-          tma_load_3d(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row);
+          tma_load_3d_hint(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row, once);
         }
         const int blk = (key0 >> p.block_shift) + (lane & 15);
         if (blk <= (min(key0 + kTile, seg.cur_hi) - 1) >> p.block_shift)
@@ -384,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         if (!(ok = warp_wait(&v_empty[s], ph, abort_flag))) break;
         if (lane == 0) {
           mbar_arrive_expect_tx(&v_full[s], kTileBytes);
-          tma_load_3d(smem + Sm::v + s * kTileBytes, &p.map[1], &v_full[s], 0, key0, row);
+          tma_load_3d_hint(smem + Sm::v + s * kTileBytes, &p.map[1], &v_full[s], 0, key0, row, once);
         }
         ++iv;
       }
