@@ -62,10 +62,10 @@ const char* swa_last_error_string(void);
 int swa_num_sms(int device);
 
 /* Failure-detection test hook; no counterpart in the reference.  While `on` is
- * non-zero, every swa_prefill_forward launch makes its first CTA withhold one
- * K/V tile load, so the MMA issuer's bounded wait for that tile runs out: the
- * launch returns with SWA_STATUS_TIMEOUT in workspace[1] after about one second,
- * having released its tensor memory, and the CUDA context stays usable.  Not for
+ * non-zero, every swa_prefill_forward and swa_kv_decode launch makes its first CTA
+ * withhold one K/V tile load, so the MMA issuer's bounded wait for that tile runs out:
+ * the launch returns with SWA_STATUS_TIMEOUT in workspace[1] (swa_kv_decode:
+ * workspace[0]) after about one second, having released its tensor memory, and the CUDA context stays usable.  Not for
  * production use; off by default. */
 void swa_test_withhold_kv_load(int on);
 

@@ -30,6 +30,7 @@ std::atomic<int> g_test_withhold{0};
 
 namespace swa {
 void set_last_error(const char* msg) { g_last_error = msg; }
+int test_withhold() { return g_test_withhold.load(); }
 }  // namespace swa
 
 extern "C" {

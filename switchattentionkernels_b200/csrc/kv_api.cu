@@ -200,6 +200,7 @@ int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const v
   p.nhb = d.nhb;
   p.ctas = d.ctas;
   p.scale_log2 = scale_log2;
+  p.test_withhold = swa::test_withhold();
   cudaError_t e = swa::launch_kv_decode(p, dtype == SWA_KV_INT8, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "KV decode launch");
   return SWA_OK;

@@ -113,6 +113,7 @@ struct __align__(64) KvDecodeParams {
   int nhb;                    // head blocks per KV head
   int ctas;
   float scale_log2;
+  int test_withhold;          // failure-detection test hook: CTA 0 withholds its second K tile
 };
 cudaError_t launch_kv_decode(const KvDecodeParams& p, bool int8, cudaStream_t stream);
 // Resident CTAs of the decode kernel per SM (what its shared memory allows).

@@ -373,7 +373,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         const uint32_t ph = ((it / kStages) & 1) ^ 1;
         const int key0 = seg.cur_lo + (seg.first + i) * kTile;
         if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
-        if (lane == 0) {
+        if (lane == 0 && !(p.test_withhold != 0 && cta == 0 && it == 1)) {
           mbar_arrive_expect_tx(&k_full[s], kTileBytes);
           tma_load_3d_hint(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row, once);
         }

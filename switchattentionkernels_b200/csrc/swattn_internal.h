@@ -164,6 +164,8 @@ uint32_t decode_smem_bytes();
 
 // Record the message returned by swa_last_error_string() on this thread.
 void set_last_error(const char* msg);
+// The failure-detection test hook's setting (swa_test_withhold_kv_load).
+int test_withhold();
 uint32_t prefill_smem_bytes();
 
 // Workspace (int32 elements) the compaction takes to split rows over several

@@ -320,6 +320,41 @@ def test_decode_repeats_bit_for_bit(cuda_device):
         assert all(torch.equal(a, b) for a, b in zip(first, got))
 
 
+@BOTH
+@pytest.mark.parametrize("B,Smax,Hq,Hkv,W", [(40, 6000, 16, 4, 300), (3, 40000, 48, 4, 2000), (6, 9000, 64, 2, 1), (2500, 130, 8, 2, 64)])
+def test_decode_many_tiles_per_cta(cuda_device, dtype, B, Smax, Hq, Hkv, W):
+    # several tiles a CTA: shares with steps for starting a unit, short and long units mixed, units that span
+    # CTAs, several head blocks; and more sequences than threads
+    g = torch.Generator().manual_seed(Smax)
+    lens = torch.randint(0, Smax + 1, (B,), generator=g)
+    lens[:2] = Smax
+    c = _filled(g, cuda_device, B, Smax, Hkv, lens, dtype=dtype, block=128)
+    q = _rows(g, B, Hq, 128, spread=0.5)
+    route = torch.rand(B, generator=g) < 0.4
+    route[0] = True
+    _check_decode(c, q, route, W, label=f"B={B} Smax={Smax} Hq={Hq} Hkv={Hkv} W={W}")
+
+
+def test_decode_wait_that_runs_out_reports_timeout(cuda_device):
+    # a withheld tile: the bounded wait gives up, the call reports it and the next one is right
+    from switchattentionkernels_b200 import _native
+    lib = _native.load()
+    g = torch.Generator().manual_seed(59)
+    c = _filled(g, cuda_device, 64, 2000, 8, [2000] * 64, dtype=E4M3, block=64, weights=False)
+    q = _rows(g, 64, 32, 128, spread=0.5).to(cuda_device)
+    route = torch.ones(64, dtype=torch.bool, device=cuda_device)
+    O, L = switch_gqa_decode_cached(q, c, route)
+    lib.swa_test_withhold_kv_load(1)
+    try:
+        with pytest.raises(RuntimeError, match="timed out"):
+            switch_gqa_decode_cached(q, c, route)
+    finally:
+        lib.swa_test_withhold_kv_load(0)
+    torch.cuda.synchronize()
+    again = switch_gqa_decode_cached(q, c, route)
+    assert torch.equal(again[0], O) and torch.equal(again[1], L)
+
+
 # --------------------------------------------------------------------------- evict
 @BOTH
 @pytest.mark.parametrize("B,Smax,Hkv,block,keep,sink,recent", [
@@ -361,6 +396,33 @@ def test_evict_matches_reference(cuda_device, dtype, B, Smax, Hkv, block, keep, 
         assert torch.equal(c.k[b, :, m:].cpu().view(torch.uint8), before["k"][b, :, m:].view(torch.uint8))
         assert torch.equal(c.v[b, :, m:].cpu().view(torch.uint8), before["v"][b, :, m:].view(torch.uint8))
         assert torch.equal(c.key_weights[b, :, m:].cpu(), before["key_weights"][b, :, m:])
+
+
+@pytest.mark.parametrize("Smax,keep", [(65536, 30000), (65537, 65536), (120000, 777), (131073, 100000), (300001, 5001)])
+def test_evict_long_sequences(cuda_device, Smax, keep):
+    # weights held by 1 to 8 CTAs, 8 or 16 a thread, and read again at every pass past 131072 rows
+    dev = cuda_device
+    g = torch.Generator().manual_seed(Smax)
+    c = make_switch_kv_cache(2, Smax, 1, device=dev, dtype=INT8, block_size=128, track_weights=True)
+    c.seq_lens.copy_(torch.tensor([Smax, Smax - 1000]))
+    w = torch.rand(2, 1, Smax, generator=g) ** 8
+    w[torch.rand(w.shape, generator=g) < 0.3] = 0.0
+    c.key_weights.copy_(w)
+    c.k.copy_(torch.randint(-127, 128, (1, 1, Smax, 128), generator=g, dtype=torch.int8).expand(2, -1, -1, -1))
+    c.v.copy_(c.k.flip(-1))
+    c.k_scale.fill_(1.0)
+    c.v_scale.fill_(0.5)
+    k, v = c.k.clone(), c.v.clone()
+    slots = switch_kv_cache_evict(c, keep=keep, sink=3, recent=100)
+    torch.cuda.synchronize()
+    for b, L in ((0, Smax), (1, Smax - 1000)):
+        mid = torch.argsort(w[b, 0, 3:L - 100], descending=True, stable=True)[:keep - 103] + 3
+        rows = torch.cat([torch.arange(3), mid.sort().values, torch.arange(L - 100, L)]) if L > keep else torch.arange(L)
+        n = rows.numel()
+        assert torch.equal(slots[b, 0, :n].cpu(), rows.to(torch.int32)) and bool((slots[b, 0, n:] == -1).all())
+        at = rows.to(dev)
+        assert torch.equal(c.k[b, 0, :n], k[b, 0, at]) and torch.equal(c.v[b, 0, :n], v[b, 0, at])
+        assert torch.equal(c.key_weights[b, 0, :n].cpu(), w[b, 0, rows]) and int(c.seq_lens[b]) == n
 
 
 @pytest.mark.parametrize("kind", ["equal", "nan", "signed", "infinite", "near"])
