@@ -701,11 +701,10 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
 // warp takes a tile at a time, with all of its scores (4 keys a lane, kHeads heads) in
 // flight at once: the pass is a chain of L2 latencies (share, sums, scores) over little data.
 constexpr int kMergeThreads = 128;
-constexpr int kWeightBlocks = 4;  // blocks over a CTA's tiles
+constexpr int kWeightBlocks = 2;  // blocks over a CTA's tiles
 
 template <int kHeads, bool kWeights>
-__global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
-  __shared__ float lse_sh[kHeads];
+__global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int c = blockIdx.x, y = blockIdx.y;
   const int units = p.Hkv * p.nhb;
@@ -772,19 +771,17 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
     return;
   }
   if constexpr (kWeights) {
-    const int wi = y * (kMergeThreads / 32) + warp;  // this warp among the share's
-    constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);
+    constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);  // warps of the share
+    int mine = y * (kMergeThreads / 32) + warp;                  // this warp's next tile, from the segment's first on
     while (seg.next(p)) {
-      const int g = seg.cur_u / p.nhb, hb0 = seg.cur_u % p.nhb;
-      if (hb0 == 0) {  // a key's tile of the first head block stands for its tiles of the others
+      const int g = seg.cur_u / p.nhb;
+      if (seg.cur_u % p.nhb != 0) continue;  // a key's tile of the first head block stands for the others' too
+      if (mine < seg.n) {
         float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
         for (int hb = 0; hb < p.nhb; ++hb) {
           const int nh = min(kHeads, p.r - hb * kHeads);
           const int t0 = seg.cur_tbase + hb * seg.cur_all;  // first tile of the unit
           const int v0 = seg.cur_vbase + sh.omega + hb * (sh.omega + seg.cur_all * kTileSteps);  // and its first step
-          const int first = share_of(v0, sh.per, sh.longer);
-          const int last = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer);
-          const int64_t slot0 = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first;
           const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + lane;
           float s[kHeads][4], old[4];
           auto load = [&](int i) {
@@ -797,37 +794,47 @@ __global__ void __launch_bounds__(kMergeThreads, 8) kv_decode_merge_kernel(const
                 s[h][j] = h < nh ? sc[(static_cast<int64_t>(i) * kHeads + h) * kTile + 32 * j] : -INFINITY;
             }
           };
-          if (wi < seg.n) load(wi);
-          __syncthreads();  // the sums of the head block before are read no more
-          for (int h = warp; h < nh; h += kMergeThreads / 32) {  // the head's lse from its segments
-            const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
-            float M = -INFINITY, L = 0.0f;
-            for (int i = lane; i <= last - first; i += 32) {
-              const float2 x = ml[static_cast<int64_t>(i) * kHeads];
-              const float mn = fmaxf(M, x.x);
-              L = fmaf(x.y, ex2_approx(x.x - mn), M == -INFINITY ? 0.0f : L * ex2_approx(M - mn));
-              M = mn;
-            }
-            const float top = warp_max(M);
-            L = M == -INFINITY && L == 0.0f ? 0.0f : L * ex2_approx(M - top);
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) L += __shfl_xor_sync(0xffffffffu, L, o);
-            if (lane == 0) lse_sh[h] = lg2_approx(L) + top;
+          load(mine);
+          // lse of head lane % kHeads from the unit's segments, 32 / kHeads of them at a time
+          const int first = share_of(v0, sh.per, sh.longer);
+          const int nseg = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer) - first + 1;
+          const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
+                             (static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first) * kHeads;
+          float M = -INFINITY, L = 0.0f;
+#pragma unroll 4
+          for (int i = lane; i < nseg * kHeads; i += 32) {
+            const float2 x = ml[i];
+            const float mn = fmaxf(M, x.x);
+            L = fmaf(x.y, ex2_approx(x.x - mn), M == -INFINITY ? L : L * ex2_approx(M - mn));
+            M = mn;
           }
-          __syncthreads();
-          for (int i = wi; i < seg.n; i += kStep) {
-            if (i != wi) load(i);
+#pragma unroll
+          for (int o = kHeads; o < 32; o <<= 1) {
+            const float mo = __shfl_xor_sync(0xffffffffu, M, o), lo = __shfl_xor_sync(0xffffffffu, L, o);
+            const float mn = fmaxf(M, mo);
+            L = (M == -INFINITY ? L : L * ex2_approx(M - mn)) + (mo == -INFINITY ? lo : lo * ex2_approx(mo - mn));
+            M = mn;
+          }
+          const float lse = lg2_approx(L) + M;
+          for (int i = mine; i < seg.n; i += kStep) {
+            if (i != mine) load(i);
+            float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) {
+              const float z = __shfl_sync(0xffffffffu, lse, h);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) w[j] += h < nh ? ex2_approx(s[h][j] - z) : 0.0f;
+            }
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-              float w = 0.0f;
-#pragma unroll
-              for (int h = 0; h < kHeads; ++h) w += h < nh ? ex2_approx(s[h][j] - lse_sh[h]) : 0.0f;
               const int key = seg.cur_lo + (seg.first + i) * kTile + 32 * j + lane;
-              if (key < seg.cur_hi) dst[key] = old[j] + w;
+              if (key < seg.cur_hi) dst[key] = old[j] + w[j];
             }
           }
         }
       }
+      mine -= seg.n;
+      while (mine < 0) mine += kStep;
     }
   }
 }
