@@ -259,7 +259,7 @@ int swa_kv_evict(const void* k_cache, const void* v_cache, const float* k_scale,
   p.keep = keep;
   p.sink = sink;
   p.recent = recent;
-  cudaError_t e = swa::launch_kv_evict(p, dtype == SWA_KV_INT8, n_same == 6, static_cast<cudaStream_t>(stream));
+  cudaError_t e = swa::launch_kv_evict(p, dtype == SWA_KV_INT8, n_same == 6, nsm, static_cast<cudaStream_t>(stream));
   if (e != cudaSuccess) return cuda_fail(e, "KV evict launch");
   return SWA_OK;
 }

@@ -70,7 +70,7 @@ struct KvEvictParams {
   int32_t* slots;             // [B, Hkv, n] written: source row of each kept row, -1 past the count
   int B, Hkv, Smax, Smax_dst, nblk, nblk_dst, block, n, keep, sink, recent;
 };
-cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, cudaStream_t stream);
+cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, int num_sms, cudaStream_t stream);
 
 // Decode over the cache.  The (sequence, KV head, head block) units' legal keys are
 // cut into tiles of 128 keys.  All units of the batch are laid end to end along one axis
