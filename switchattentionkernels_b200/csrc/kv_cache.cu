@@ -468,30 +468,34 @@ cudaError_t launch_select(const KvEvictParams& p, int num_sms, cudaStream_t stre
 // ---------------------------------------------------------------------------
 // evict: move
 // ---------------------------------------------------------------------------
-// A CTA gathers 128 destination rows of one (sequence, KV head), K and V, into
-// registers (8 x 16 bytes per thread), then rounds them to their destination
+// A CTA gathers kRows destination rows of one (sequence, KV head), K and V, into
+// registers (8 x 16 bytes per thread, 2 kRows threads), then rounds them to their destination
 // block's scale (the largest of its rows' scales: rows of that scale keep their
 // bytes) and stores them.  HBM-bound: each kept row is read and written once.
 //   Out of place: one CTA per 128 rows.
-//   In place: a cluster of 8 CTAs walks over the rows of its (sequence, KV head)
-//   1024 at a time; all eight have read their rows before any of them writes.  A
-//   kept row's source lies at or behind its destination, so a later step's sources
-//   (rows and scales) are never behind an earlier step's stores.
-constexpr int kMoveThreads = 256;
+//   In place: a cluster of 8 CTAs walks over the rows of its (sequence, KV head) 8 kRows
+//   at a time; all eight have read their rows before any of them writes.  A kept row's
+//   source lies at or behind its destination, so a later step's sources (rows and scales)
+//   are never behind an earlier step's stores.  A step is a chain of some 4 us (slots, rows,
+//   barrier).  Where it takes several, and the clusters of all (sequence, KV head)s fit on the SMs at
+//   once, a CTA takes kBigRows rows a step (a whole SM's registers), else kMoveRows, so that several
+//   clusters share the SMs.  Whole evictions in place, 512 / 128 rows: 2 x 131K rows of 4 heads
+//   to 8K 36 / 55 us, 16 x 8K rows of 8 heads to 2K 65 / 37 us.
 constexpr int kMoveRows = 128;
+constexpr int kBigRows = 512;
 constexpr int kMoveCluster = 8;
 
-template <bool kInt8, bool kInPlace>
-__device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, int base, bool sync_cluster) {
-  __shared__ int slot_sh[kMoveRows];
-  __shared__ float scale_sh[2][kMoveRows];
-  __shared__ float warp_max[2][kMoveRows / 32];
+template <bool kInt8, bool kInPlace, int kRows>
+__device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, int base) {
+  __shared__ int slot_sh[kRows];
+  __shared__ float scale_sh[2][kRows];
+  __shared__ float warp_max[2][kRows / 32];
   const int tid = threadIdx.x;
   // -1: no row, here or further on
   int slot = -1;
   float s[2] = {0.0f, 0.0f}, weight = 0.0f;
   bool moved = false;
-  if (tid < kMoveRows) {
+  if (tid < kRows) {
     const int row = base + tid;
     if (row < p.n) slot = p.slots[unit * p.n + row];
     moved = slot != row && slot >= 0;
@@ -507,14 +511,14 @@ __device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, 
   if (work) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = 32 * (i & 3) + (tid >> 3);
+      const int r = kRows / 4 * (i & 3) + (tid >> 3);
       const int src = slot_sh[r];
       v[i] = make_uint4(0, 0, 0, 0);
       if (src >= 0)  // (read once: the streaming load measured 5 % faster than a plain one)
         v[i] = __ldcs(reinterpret_cast<const uint4*>(p.src[i >> 2] + (unit * p.Smax + src) * 128 + 16 * (tid & 7)));
     }
     // destination scale of each row: the maximum over its block
-    if (tid < kMoveRows) {
+    if (tid < kRows) {
       float m[2] = {s[0], s[1]};
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
@@ -528,7 +532,7 @@ __device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, 
     }
     __syncthreads();
     float d[2] = {0.0f, 0.0f};
-    if (tid < kMoveRows) {
+    if (tid < kRows) {
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) {
         d[kv] = scale_sh[kv][tid];
@@ -539,13 +543,13 @@ __device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, 
       }
     }
     __syncthreads();
-    if (tid < kMoveRows) {
+    if (tid < kRows) {
 #pragma unroll
       for (int kv = 0; kv < 2; ++kv) scale_sh[kv][tid] = s[kv] == d[kv] ? 1.0f : s[kv] / d[kv];
     }
     __syncthreads();
-    if (kInPlace && sync_cluster) cg::this_cluster().sync();
-    if (tid < kMoveRows && slot >= 0) {
+    if (kInPlace) cg::this_cluster().sync();
+    if (tid < kRows && slot >= 0) {
       const int row = base + tid;
       p.dst_weights[unit * p.Smax_dst + row] = weight;
       if (tid % p.block == 0) {
@@ -555,13 +559,13 @@ __device__ __forceinline__ void move_rows(const KvEvictParams& p, int64_t unit, 
     }
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const int r = 32 * (i & 3) + (tid >> 3);
+      const int r = kRows / 4 * (i & 3) + (tid >> 3);
       if (slot_sh[r] < 0) continue;
       const float ratio = scale_sh[i >> 2][r];
       const uint4 o = ratio == 1.0f ? v[i] : rescale8<kInt8>(v[i], ratio);
       *reinterpret_cast<uint4*>(p.dst[i >> 2] + (unit * p.Smax_dst + base + r) * 128 + 16 * (tid & 7)) = o;
     }
-  } else if (kInPlace && sync_cluster) {
+  } else if (kInPlace) {
     cg::this_cluster().sync();
   }
 }
@@ -574,22 +578,22 @@ __device__ __forceinline__ void write_kept_length(const KvEvictParams& p, int64_
 }
 
 template <bool kInt8>
-__global__ void __launch_bounds__(kMoveThreads) kv_move_kernel(const __grid_constant__ KvEvictParams p, int tiles) {
+__global__ void __launch_bounds__(2 * kMoveRows) kv_move_kernel(const __grid_constant__ KvEvictParams p, int tiles) {
   const int64_t unit = blockIdx.x / tiles;
   const int tile = blockIdx.x % tiles;
   cudaGridDependencySynchronize();
-  move_rows<kInt8, false>(p, unit, tile * kMoveRows, false);
+  move_rows<kInt8, false, kMoveRows>(p, unit, tile * kMoveRows);
   if (tile == 0) write_kept_length(p, unit);
 }
 
-template <bool kInt8>
-__global__ void __launch_bounds__(kMoveThreads)
+template <bool kInt8, int kRows>
+__global__ void __launch_bounds__(2 * kRows)
     kv_move_in_place_kernel(const __grid_constant__ KvEvictParams p) {
   const int64_t unit = blockIdx.x / kMoveCluster;
   const int rank = blockIdx.x % kMoveCluster;
   cudaGridDependencySynchronize();
-  for (int step = 0; step < p.n; step += kMoveCluster * kMoveRows) {
-    move_rows<kInt8, true>(p, unit, step + rank * kMoveRows, true);
+  for (int step = 0; step < p.n; step += kMoveCluster * kRows) {
+    move_rows<kInt8, true, kRows>(p, unit, step + rank * kRows);
     __syncthreads();
   }
   if (rank == 0) write_kept_length(p, unit);
@@ -608,11 +612,16 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, in
   cudaError_t e = launch_select(p, num_sms, stream);
   if (e != cudaSuccess) return e;
   const int units = p.B * p.Hkv;
-  if (in_place)
-    return launch_cluster_dependent(kMoveCluster, int8 ? kv_move_in_place_kernel<true> : kv_move_in_place_kernel<false>,
-                                    dim3(units * kMoveCluster), dim3(kMoveThreads), 0, stream, p);
+  if (in_place) {
+    const bool big = units * kMoveCluster <= num_sms && p.n > kMoveCluster * kMoveRows;
+    void (*kernel)(KvEvictParams) =
+        big ? (int8 ? kv_move_in_place_kernel<true, kBigRows> : kv_move_in_place_kernel<false, kBigRows>)
+            : (int8 ? kv_move_in_place_kernel<true, kMoveRows> : kv_move_in_place_kernel<false, kMoveRows>);
+    return launch_cluster_dependent(kMoveCluster, kernel, dim3(units * kMoveCluster), dim3(2 * (big ? kBigRows : kMoveRows)), 0,
+                                    stream, p);
+  }
   const int tiles = (p.n + kMoveRows - 1) / kMoveRows;
-  return launch_dependent(int8 ? kv_move_kernel<true> : kv_move_kernel<false>, dim3(units * tiles), dim3(kMoveThreads), 0,
+  return launch_dependent(int8 ? kv_move_kernel<true> : kv_move_kernel<false>, dim3(units * tiles), dim3(2 * kMoveRows), 0,
                           stream, p, tiles);
 }
 

@@ -361,6 +361,7 @@ def test_decode_wait_that_runs_out_reports_timeout(cuda_device):
     (1, 64, 1, 16, 1, 0, 0), (3, 100, 2, 16, 40, 4, 10), (2, 1000, 3, 64, 300, 0, 0), (4, 777, 2, 32, 500, 0, 500),
     (2, 5000, 2, 128, 1111, 7, 300), (3, 300, 1, 64, 300, 5, 5), (2, 300, 1, 64, 10 ** 12, 5, 5), (2, 9000, 1, 64, 4097, 1, 33),
     (1, 40000, 1, 16, 9000, 3, 1000), (2, 600, 2, 128, 130, 130, 0), (40, 50, 2, 16, 20, 2, 3),
+    (10, 2000, 2, 64, 1500, 4, 64),
 ])
 def test_evict_matches_reference(cuda_device, dtype, B, Smax, Hkv, block, keep, sink, recent):
     dev = cuda_device
