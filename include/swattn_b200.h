@@ -336,7 +336,8 @@ int swa_prefill_forward_noalloc(const void* q, const void* k, const void* v, con
  * strides[1] + g * strides[2] + d (host arrays of 3 element strides, multiples of 8),
  * 0 <= t < T.  Rows t < n_b (new_lens[b] clamped to [0, T]; new_lens NULL: T) of sequence
  * b become cache rows start[b] + t (those at Smax and past it are dropped), and
- * seq_lens[b] the end of them; start may be seq_lens.  Each touched block's scale
+ * seq_lens[b] the end of them; start and new_lens may be seq_lens, but may not overlap it
+ * otherwise.  Each touched block's scale
  * becomes the smallest power of two (at least 2^-126; 0 for a block of zeros) that both
  * its earlier rows' scale and the largest finite |value| of its new rows need (448 /
  * 127 times it reaches them); earlier rows of the block are rounded again when it

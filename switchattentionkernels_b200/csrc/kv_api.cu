@@ -89,6 +89,7 @@ int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides
     return fail(SWA_E_INVALID, "null pointer");
   if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache))
     return fail(SWA_E_INVALID, "k/v and the caches must be 16-byte aligned");
+  if (k_cache == v_cache || k_scale == v_scale) return fail(SWA_E_INVALID, "K and V must not share a cache");
   for (int i = 0; i < 3; ++i)
     if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
       return fail(SWA_E_INVALID, "strides of k/v must be multiples of 8 elements");
@@ -222,6 +223,7 @@ int swa_kv_evict(const void* k_cache, const void* v_cache, const float* k_scale,
     return fail(SWA_E_INVALID, "null pointer");
   if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_out) || !aligned16(v_out))
     return fail(SWA_E_INVALID, "the caches must be 16-byte aligned");
+  if (k_out == v_out || k_scale_out == v_scale_out) return fail(SWA_E_INVALID, "K and V must not share a cache");
   const int n = std::min(keep, Smax);
   if (Smax_out < n) return fail(SWA_E_INVALID, "the destination holds fewer rows than are kept");
   const bool same[6] = {k_cache == k_out, v_cache == v_out, k_scale == k_scale_out, v_scale == v_scale_out,

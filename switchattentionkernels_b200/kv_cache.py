@@ -165,7 +165,8 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     they are.  ``new_lens``: int32 ``[B]``, the rows of a padded batch that count (default:
     all ``T``).  ``start``: int32 ``[B]``, the row at which each sequence's new rows begin
     (default ``cache.seq_lens``; earlier: the rows from there on are replaced, e.g. after
-    rejected draft tokens).  Rows that do not fit (``>= Smax``) are dropped.
+    rejected draft tokens).  Neither may overlap ``cache.seq_lens`` unless it is that tensor.
+    Rows that do not fit (``>= Smax``) are dropped.
 
     A block's scale is the smallest power of two that its rows need, and only grows:
     when it does, the block's earlier rows are rounded again.  Rounding is to nearest

@@ -127,18 +127,18 @@ def test_c_abi_refusals():
     lib = _native.load()
     st = (ctypes.c_int64 * 3)(256, 256, 128)
     odd = (ctypes.c_int64 * 3)(256, 256, 4)
-    one = ctypes.c_void_p(256)
+    one, two, three, four = (ctypes.c_void_p(x) for x in (256, 512, 768, 1024))
     none = None
 
-    def append(k=one, v=one, ks=st, B=1, T=1, H=1, S=16, D=128, block=16, dtype=1, start=one, lens=one):
-        return lib.swa_kv_append(k, v, ks, st, start, none, one, one, one, one, none, lens, B, T, H, S, D, block, dtype, none)
+    def append(k=one, v=one, ks=st, B=1, T=1, H=1, S=16, D=128, block=16, dtype=1, start=one, new=none, vc=two, vs=four, lens=one):
+        return lib.swa_kv_append(k, v, ks, st, start, new, one, vc, three, vs, none, lens, B, T, H, S, D, block, dtype, none)
 
     def decode(q=one, sb=128, B=1, S=16, Hq=2, H=1, D=128, block=16, window=4, scale=1.0, dtype=1, ws=one, nbytes=0):
         return lib.swa_kv_decode(q, sb, 128, one, one, one, one, one, one, one, one, none, B, S, Hq, H, D, block, window, scale,
                                  dtype, ws, nbytes, none)
 
-    def evict(k=one, ko=one, B=1, H=1, S=16, So=16, D=128, block=16, keep=4, sink=0, recent=0, dtype=1):
-        return lib.swa_kv_evict(k, one, one, one, one, one, ko, one, one, one, one, one, one, B, H, S, So, D, block, keep, sink,
+    def evict(k=one, ko=one, vo=two, vs=four, B=1, H=1, S=16, So=16, D=128, block=16, keep=4, sink=0, recent=0, dtype=1):
+        return lib.swa_kv_evict(k, two, three, four, one, one, ko, vo, three, vs, one, one, one, B, H, S, So, D, block, keep, sink,
                                 recent, dtype, none)
 
     invalid, unsupported = -1, -3
@@ -147,7 +147,8 @@ def test_c_abi_refusals():
                decode(q=ctypes.c_void_p(4)), decode(sb=4), decode(B=0), decode(Hq=3, H=2), decode(Hq=0), decode(window=0),
                decode(scale=0.0), decode(scale=math.nan), decode(block=8), decode(dtype=3), decode(ws=none), evict(k=none),
                evict(keep=0), evict(sink=-1), evict(keep=4, sink=3, recent=2), evict(S=0), evict(dtype=9),
-               evict(ko=ctypes.c_void_p(512)), evict(So=3), evict(So=17)):
+               evict(ko=ctypes.c_void_p(2048)), evict(So=3), evict(So=17), append(vc=one), append(vs=three), evict(vo=one),
+               evict(vs=three), append(B=4, start=ctypes.c_void_p(260)), append(B=4, new=ctypes.c_void_p(252))):
         assert rc == invalid
     for rc in (append(D=64), decode(D=256), evict(D=1), append(B=70000, T=2), append(H=40000, T=2), append(S=(1 << 30) + 1)):
         assert rc == unsupported
