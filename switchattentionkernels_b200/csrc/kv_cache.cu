@@ -56,8 +56,15 @@ __device__ __forceinline__ uint32_t pack8(float a, float b, float c, float d) {
 template <bool kInt8>
 __device__ __forceinline__ uint32_t rescale8(uint32_t v, float ratio) {
   if constexpr (kInt8) {
-    auto x = [v, ratio](int i) { return static_cast<float>(static_cast<int8_t>(v >> (8 * i))) * ratio; };
-    return pack8<true>(x(0), x(1), x(2), x(3));
+    // a byte (offset by 128) as the low byte of 2^23 makes the float 2^23 + 128 + value, and the sum with
+    // 1.5 * 2^23 rounds the product to a whole number in its low byte: no conversion instructions,
+    // which run at a quarter of the rate (an eviction that rescales most rows: 28.8 -> 24.2 us)
+    const uint32_t u = v ^ 0x80808080u;
+    auto x = [u, ratio](uint32_t sel) {
+      const float f = __uint_as_float(__byte_perm(u, 0x4B000000u, sel)) - 8388736.0f;
+      return __float_as_uint(fmaf(fmaxf(f, -127.0f), ratio, 12582912.0f));
+    };
+    return __byte_perm(__byte_perm(x(0x7440), x(0x7441), 0x0040), __byte_perm(x(0x7442), x(0x7443), 0x0040), 0x5410);
   } else {
     uint32_t lo, hi;
     e4m3x4_to_f16x2x2(v, lo, hi);
@@ -319,10 +326,8 @@ cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
 // Latency-bound (a chain of a dozen barriers over little data), so the weights are
 // read once and stay in registers, kPerThread of them a thread; with kPerThread = 0
 // (more rows than 8 CTAs can hold) every pass reads them again, from L2.
-constexpr int kSelThreads = 1024;
 constexpr int kSelMaxCluster = 8;
 constexpr int kSelBins = 2048;
-constexpr int kSelWarps = kSelThreads / 32;
 
 // Order-preserving integer form of a weight; NaN below everything, -0 equal to +0.
 __device__ __forceinline__ uint32_t order_bits(float w) {
@@ -331,8 +336,10 @@ __device__ __forceinline__ uint32_t order_bits(float w) {
   return u ^ ((u >> 31) != 0u ? 0xFFFFFFFFu : 0x80000000u);
 }
 
-template <int kPerThread>
+template <int kSelThreads, int kPerThread>
 __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_constant__ KvEvictParams p) {
+  constexpr int kSelWarps = kSelThreads / 32;
+  constexpr int kPer = kSelBins / kSelThreads;  // bins of a thread
   __shared__ uint32_t hist[3][kSelBins];
   __shared__ uint32_t warp_sum[kSelWarps];
   __shared__ uint32_t found[2];
@@ -393,14 +400,20 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
         if (i < w1 && i >= lo && i < hi && (pass == 0 || (u >> up) == pfx)) atomicAdd(&hist[pass][(u >> shift) & dmask], 1u);
       });
       if (ncta > 1) cluster.sync(); else __syncthreads();
-      // bins 2 tid and 2 tid + 1 over the whole cluster, then the sum of the bins above them
-      uint2 mine = make_uint2(0, 0);
+      // bins kPer tid .. over the whole cluster, then the sum of the bins above them
+      uint32_t bin[kPer] = {};
       for (int r = 0; r < ncta; ++r) {
-        const uint2 h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[pass][0], r))[tid];
-        mine.x += h.x;
-        mine.y += h.y;
+        const uint2* h = reinterpret_cast<const uint2*>(cluster.map_shared_rank(&hist[pass][0], r)) + tid * (kPer / 2);
+#pragma unroll
+        for (int j = 0; j < kPer / 2; ++j) {
+          const uint2 x = h[j];
+          bin[2 * j] += x.x;
+          bin[2 * j + 1] += x.y;
+        }
       }
-      const uint32_t total = mine.x + mine.y;
+      uint32_t total = 0;
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) total += bin[j];
       uint32_t suffix = total;  // over this lane and the lanes above it
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -409,12 +422,17 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
       }
       if (lane == 0) warp_sum[warp] = suffix;
       __syncthreads();
-      uint32_t above = __reduce_add_sync(0xffffffffu, lane > warp ? warp_sum[lane] : 0u) + suffix - total;
+      uint32_t above =
+          __reduce_add_sync(0xffffffffu, lane > warp && lane < kSelWarps ? warp_sum[lane] : 0u) + suffix - total;
       if (above < need && above + total >= need) {  // exactly one thread
-        const bool top = above + mine.y >= need;
-        if (!top) above += mine.y;
-        found[0] = static_cast<uint32_t>(2 * tid + (top ? 1 : 0));
-        found[1] = need - above;
+#pragma unroll
+        for (int j = kPer - 1; j >= 0; --j) {
+          if (above < need && above + bin[j] >= need) {
+            found[0] = static_cast<uint32_t>(kPer * tid + j);
+            found[1] = need - above;
+          }
+          above += bin[j];
+        }
       }
       __syncthreads();
       pfx = (pfx << (pass == 2 ? 10 : 11)) | found[0];
@@ -467,19 +485,25 @@ __global__ void __launch_bounds__(kSelThreads) kv_select_kernel(const __grid_con
   });
 }
 
-// CTAs per (sequence, KV head), from the most rows a sequence can have: as few as hold them
-// with 8 weights a thread where that fills at most the SMs once (a CTA takes a whole
-// SM), else with 16.  Measured, whole evictions of 32K rows, 8 against 16: 32 (sequence,
-// KV head)s 35.7 / 39.3 us, 256 of them 155 / 118 us.  Past 8 x 16 x 1024 rows no weight is held.
+// CTAs per (sequence, KV head), from the most rows a sequence can have.  Up to 2048 rows one
+// CTA of 256 threads, several of which share an SM; more rows: CTAs of 1024 threads, each a
+// whole SM, as few as hold the rows with 8 weights a thread where that fills at most the SMs once,
+// else with 16.  Past 8 x 16 x 1024 rows no weight is held.  Measured, whole evictions: 512
+// (sequence, KV head)s of 256 rows 29.1 us with 1024 threads, 13.0 us with 256; 32K rows with 8 against
+// 16 weights a thread, 32 of them 35.7 / 39.3 us, 256 of them 155 / 118 us.
 cudaError_t launch_select(const KvEvictParams& p, int num_sms, cudaStream_t stream) {
   const int64_t units = static_cast<int64_t>(p.B) * p.Hkv;
-  int cluster = 1;
-  while (cluster < kSelMaxCluster && p.Smax > cluster * kSelThreads * 8) cluster *= 2;
-  if (cluster > 1 && units * cluster > num_sms && p.Smax <= cluster / 2 * kSelThreads * 16) cluster /= 2;
-  void (*kernel)(KvEvictParams) = p.Smax <= cluster * kSelThreads * 8    ? kv_select_kernel<8>
-                                  : p.Smax <= cluster * kSelThreads * 16 ? kv_select_kernel<16>
-                                                                         : kv_select_kernel<0>;
-  return launch_cluster_dependent(cluster, kernel, dim3(static_cast<unsigned>(units * cluster)), dim3(kSelThreads), 0, stream, p);
+  int cluster = 1, threads = 256;
+  void (*kernel)(KvEvictParams) = kv_select_kernel<256, 8>;
+  if (p.Smax > 256 * 8) {
+    threads = 1024;
+    while (cluster < kSelMaxCluster && p.Smax > cluster * 1024 * 8) cluster *= 2;
+    if (cluster > 1 && units * cluster > num_sms && p.Smax <= cluster / 2 * 1024 * 16) cluster /= 2;
+    kernel = p.Smax <= cluster * 1024 * 8    ? kv_select_kernel<1024, 8>
+             : p.Smax <= cluster * 1024 * 16 ? kv_select_kernel<1024, 16>
+                                             : kv_select_kernel<1024, 0>;
+  }
+  return launch_cluster_dependent(cluster, kernel, dim3(static_cast<unsigned>(units * cluster)), dim3(threads), 0, stream, p);
 }
 
 // ---------------------------------------------------------------------------
