@@ -565,6 +565,51 @@ def test_two_streams_at_once(cuda_device):
             assert torch.equal(getattr(c, n).view(torch.uint8), getattr(mine, n).view(torch.uint8)), n
 
 
+def test_captured_behind_a_memset_and_a_join(cuda_device):
+    # the dependent launches in a graph whose nodes before them are a memset, a copy and another stream's
+    # work, replayed several times; and two graphs over the same caches replayed one after the other
+    from switchattentionkernels_b200 import _core
+    dev = cuda_device
+    g = torch.Generator().manual_seed(83)
+    c = _filled(g, dev, 2, 3000, 2, [2900, 1700], dtype=E4M3, block=64)
+    k, v, q = (_rows(g, 2, h, 128, spread=0.4).to(dev) for h in (2, 2, 8))
+    route = torch.tensor([True, False], device=dev)
+    out = make_switch_kv_cache(2, 1000, 2, device=dev, block_size=64, track_weights=True)
+    lens0, w0 = c.seq_lens.clone(), c.key_weights.clone()
+    side = torch.cuda.Stream()
+
+    def step():
+        out.k.view(torch.uint8).zero_()
+        c.seq_lens.copy_(lens0)
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            c.key_weights.copy_(w0)
+            kk = k * 2
+        main.wait_stream(side)
+        switch_kv_cache_append(c, kk, v)
+        O, L = switch_gqa_decode_cached(q, c, route, window_size=500)
+        return O, L, switch_kv_cache_evict(c, keep=900, sink=4, recent=100, out=out), c.key_weights.clone(), out.v.view(torch.uint8).clone()
+
+    check, _core.CHECK_DEVICE_STATUS = _core.CHECK_DEVICE_STATUS, False
+    try:
+        want = step()
+        torch.cuda.synchronize()
+        graphs = []
+        for _ in range(2):
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                got = step()
+            graphs.append((graph, got))
+    finally:
+        _core.CHECK_DEVICE_STATUS = check
+    for _ in range(3):
+        for graph, got in graphs:
+            graph.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_rows_past_four_gigabytes(cuda_device):
     # each head's rows take more than 2^31 bytes, the two together more than 2^32
     dev = cuda_device
