@@ -787,62 +787,57 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
     while (seg.next(p)) {
       const int g = seg.cur_u / p.nhb;
       if (seg.cur_u % p.nhb != 0) continue;  // a key's tile of the first head block stands for the others' too
-      if (mine < seg.n) {
-        float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
+      float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
+      float lse = 0.0f;  // of head lane % kHeads of head block `of`
+      int of = -1;
+      for (int i = mine; i < seg.n; i += kStep) {
+        const int key0 = seg.cur_lo + (seg.first + i) * kTile + lane;
+        float old[4], w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) old[j] = key0 + 32 * j < seg.cur_hi ? dst[key0 + 32 * j] : 0.0f;
         for (int hb = 0; hb < p.nhb; ++hb) {
           const int nh = min(kHeads, p.r - hb * kHeads);
-          const int t0 = seg.cur_tbase + hb * seg.cur_all;  // first tile of the unit
-          const int v0 = seg.cur_vbase + sh.omega + hb * (sh.omega + seg.cur_all * kTileSteps);  // and its first step
-          const float* sc = p.scores + static_cast<int64_t>(t0 + seg.first) * kHeads * kTile + lane;
-          float s[kHeads][4], old[4];
-          auto load = [&](int i) {
+          const float* sc = p.scores + static_cast<int64_t>(seg.cur_tbase + hb * seg.cur_all + seg.first + i) * kHeads * kTile + lane;
+          float s[kHeads][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int key = seg.cur_lo + (seg.first + i) * kTile + 32 * j + lane;
-              old[j] = key < seg.cur_hi ? dst[key] : 0.0f;
+          for (int h = 0; h < kHeads; ++h) {
 #pragma unroll
-              for (int h = 0; h < kHeads; ++h)
-                s[h][j] = h < nh ? sc[(static_cast<int64_t>(i) * kHeads + h) * kTile + 32 * j] : -INFINITY;
-            }
-          };
-          load(mine);
-          // lse of head lane % kHeads from the unit's segments, 32 / kHeads of them at a time
-          const int first = share_of(v0, sh.per, sh.longer);
-          const int nseg = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer) - first + 1;
-          const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
-                             (static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first) * kHeads;
-          float M = -INFINITY, L = 0.0f;
+            for (int j = 0; j < 4; ++j) s[h][j] = h < nh ? sc[h * kTile + 32 * j] : -INFINITY;
+          }
+          if (of != hb) {  // from the unit's segments, 32 / kHeads of them at a time
+            of = hb;
+            const int v0 = seg.cur_vbase + sh.omega + hb * (sh.omega + seg.cur_all * kTileSteps);  // the unit's first tile
+            const int first = share_of(v0, sh.per, sh.longer);
+            const int nseg = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer) - first + 1;
+            const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
+                               (static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first) * kHeads;
+            float M = -INFINITY, L = 0.0f;
 #pragma unroll 4
-          for (int i = lane; i < nseg * kHeads; i += 32) {
-            const float2 x = ml[i];
-            const float mn = fmaxf(M, x.x);
-            L = fmaf(x.y, ex2_approx(x.x - mn), M == -INFINITY ? L : L * ex2_approx(M - mn));
-            M = mn;
-          }
-#pragma unroll
-          for (int o = kHeads; o < 32; o <<= 1) {
-            const float mo = __shfl_xor_sync(0xffffffffu, M, o), lo = __shfl_xor_sync(0xffffffffu, L, o);
-            const float mn = fmaxf(M, mo);
-            L = (M == -INFINITY ? L : L * ex2_approx(M - mn)) + (mo == -INFINITY ? lo : lo * ex2_approx(mo - mn));
-            M = mn;
-          }
-          const float lse = lg2_approx(L) + M;
-          for (int i = mine; i < seg.n; i += kStep) {
-            if (i != mine) load(i);
-            float w[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int h = 0; h < kHeads; ++h) {
-              const float z = __shfl_sync(0xffffffffu, lse, h);
-#pragma unroll
-              for (int j = 0; j < 4; ++j) w[j] += h < nh ? ex2_approx(s[h][j] - z) : 0.0f;
+            for (int k = lane; k < nseg * kHeads; k += 32) {
+              const float2 x = ml[k];
+              const float mn = fmaxf(M, x.x);
+              L = fmaf(x.y, ex2_approx(x.x - mn), M == -INFINITY ? L : L * ex2_approx(M - mn));
+              M = mn;
             }
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const int key = seg.cur_lo + (seg.first + i) * kTile + 32 * j + lane;
-              if (key < seg.cur_hi) dst[key] = old[j] + w[j];
+            for (int o = kHeads; o < 32; o <<= 1) {
+              const float mo = __shfl_xor_sync(0xffffffffu, M, o), lo = __shfl_xor_sync(0xffffffffu, L, o);
+              const float mn = fmaxf(M, mo);
+              L = (M == -INFINITY ? L : L * ex2_approx(M - mn)) + (mo == -INFINITY ? lo : lo * ex2_approx(mo - mn));
+              M = mn;
             }
+            lse = lg2_approx(L) + M;
+          }
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) {
+            const float z = __shfl_sync(0xffffffffu, lse, h);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) w[j] += h < nh ? ex2_approx(s[h][j] - z) : 0.0f;
           }
         }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (key0 + 32 * j < seg.cur_hi) dst[key0 + 32 * j] = old[j] + w[j];
       }
       mine -= seg.n;
       while (mine < 0) mine += kStep;

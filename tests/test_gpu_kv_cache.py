@@ -321,7 +321,7 @@ def test_decode_repeats_bit_for_bit(cuda_device):
 
 
 @BOTH
-@pytest.mark.parametrize("B,Smax,Hq,Hkv,W", [(40, 6000, 16, 4, 300), (3, 40000, 48, 4, 2000), (6, 9000, 64, 2, 1), (2500, 130, 8, 2, 64)])
+@pytest.mark.parametrize("B,Smax,Hq,Hkv,W", [(40, 6000, 16, 4, 300), (3, 40000, 48, 4, 2000), (5, 700, 72, 3, 129), (6, 9000, 64, 2, 1), (2500, 130, 8, 2, 64)])
 def test_decode_many_tiles_per_cta(cuda_device, dtype, B, Smax, Hq, Hkv, W):
     # several tiles a CTA: shares with steps for starting a unit, short and long units mixed, units that span
     # CTAs, several head blocks; and more sequences than threads
