@@ -332,9 +332,8 @@ int swa_prefill_forward_noalloc(const void* q, const void* k, const void* v, con
 #define SWA_KV_E4M3 1
 #define SWA_KV_INT8 2
 
-/* Appends rows.  k_new / v_new: bf16, element (b, t, g, d) at b * strides[0] + t *
- * strides[1] + g * strides[2] + d (host arrays of 3 element strides, multiples of 8),
- * 0 <= t < T.  Rows t < n_b (new_lens[b] clamped to [0, T]; new_lens NULL: T) of sequence
+/* Appends rows.  k_new / v_new: bf16, element (b, t, g, d) at b * stride_b + t *
+ * stride_t + g * stride_h + d (strides in elements, multiples of 8), 0 <= t < T.  Rows t < n_b (new_lens[b] clamped to [0, T]; new_lens NULL: T) of sequence
  * b become cache rows start[b] + t (those at Smax and past it are dropped), and
  * seq_lens[b] the end of them; start and new_lens may be seq_lens, but may not overlap it
  * otherwise.  Each touched block's scale
@@ -343,8 +342,8 @@ int swa_prefill_forward_noalloc(const void* q, const void* k, const void* v, con
  * 127 times it reaches them); earlier rows of the block are rounded again when it
  * differs from what it was.  Values are rounded to nearest even; infinities saturate,
  * NaN stays NaN (e4m3) or becomes 0 (int8).  key_weights (nullable): new rows start at 0. */
-int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides, const int64_t* v_strides,
-                  const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
+int swa_kv_append(const void* k_new, const void* v_new, int64_t k_stride_b, int64_t k_stride_t, int64_t k_stride_h,
+                  int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
                   float* v_scale, float* key_weights, int32_t* seq_lens, int B, int T, int Hkv, int Smax,
                   int head_dim, int block_size, int dtype, void* stream);
 

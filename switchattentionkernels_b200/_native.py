@@ -177,7 +177,7 @@ def _declare(lib) -> None:
     _i64 = ctypes.c_int64
     lib.swa_kv_append.restype = _i
     lib.swa_kv_append.argtypes = [
-        _p, _p, ctypes.POINTER(_i64), ctypes.POINTER(_i64),  # k_new, v_new, k_strides[3], v_strides[3]
+        _p, _p, _i64, _i64, _i64, _i64, _i64, _i64,  # k_new, v_new, strides (b, t, g) of each
         _p, _p,                # start, new_lens
         _p, _p, _p, _p, _p, _p,  # k_cache, v_cache, k_scale, v_scale, key_weights, seq_lens
         _i, _i, _i, _i, _i, _i, _i,  # B, T, Hkv, Smax, head_dim, block_size, dtype

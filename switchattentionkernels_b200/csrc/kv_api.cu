@@ -76,22 +76,23 @@ KvDecodePlan plan_decode(int B, int Smax, int Hq, int Hkv, bool weights, int nsm
 
 extern "C" {
 
-int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides, const int64_t* v_strides,
-                  const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
+int swa_kv_append(const void* k_new, const void* v_new, int64_t k_stride_b, int64_t k_stride_t, int64_t k_stride_h,
+                  int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
                   float* v_scale, float* key_weights, int32_t* seq_lens, int B, int T, int Hkv, int Smax,
                   int head_dim, int block_size, int dtype, void* stream) {
   if (head_dim != 128) return fail(SWA_E_UNSUPPORTED, "head_dim must be 128");
   int rc = check_cache(dtype, B, Hkv, Smax, block_size);
   if (rc != SWA_OK) return rc;
   if (T <= 0) return fail(SWA_E_INVALID, "empty or negative shape");
-  if (k_new == nullptr || v_new == nullptr || k_strides == nullptr || v_strides == nullptr || start == nullptr ||
+  if (k_new == nullptr || v_new == nullptr || start == nullptr ||
       k_cache == nullptr || v_cache == nullptr || k_scale == nullptr || v_scale == nullptr || seq_lens == nullptr)
     return fail(SWA_E_INVALID, "null pointer");
   if (!aligned16(k_new) || !aligned16(v_new) || !aligned16(k_cache) || !aligned16(v_cache))
     return fail(SWA_E_INVALID, "k/v and the caches must be 16-byte aligned");
   if (k_cache == v_cache || k_scale == v_scale) return fail(SWA_E_INVALID, "K and V must not share a cache");
-  for (int i = 0; i < 3; ++i)
-    if (k_strides[i] % 8 != 0 || v_strides[i] % 8 != 0)
+  const int64_t strides[2][3] = {{k_stride_b, k_stride_t, k_stride_h}, {v_stride_b, v_stride_t, v_stride_h}};
+  for (const auto& s : strides)
+    if (s[0] % 8 != 0 || s[1] % 8 != 0 || s[2] % 8 != 0)
       return fail(SWA_E_INVALID, "strides of k/v must be multiples of 8 elements");
   for (const int32_t* t : {start, new_lens})
     if (t != nullptr && t != seq_lens && t < seq_lens + B && seq_lens < t + B)
@@ -104,7 +105,6 @@ int swa_kv_append(const void* k_new, const void* v_new, const int64_t* k_strides
   swa::KvAppendParams p{};
   p.x[0] = static_cast<const __nv_bfloat16*>(k_new);
   p.x[1] = static_cast<const __nv_bfloat16*>(v_new);
-  const int64_t* strides[2] = {k_strides, v_strides};
   for (int kv = 0; kv < 2; ++kv) {
     p.sb[kv] = strides[kv][0];
     p.st[kv] = strides[kv][1];

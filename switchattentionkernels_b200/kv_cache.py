@@ -17,8 +17,6 @@ never synchronise and can be captured into a CUDA graph.
 """
 from __future__ import annotations
 
-import ctypes
-from contextlib import nullcontext
 from dataclasses import dataclass
 from functools import lru_cache
 
@@ -29,7 +27,6 @@ from ._core import LOG2E
 
 HEAD_DIM = 128
 BLOCK_SIZES = (16, 32, 64, 128)
-_Strides = ctypes.c_int64 * 3
 _DTYPES = {torch.float8_e4m3fn: _native.KV_E4M3, torch.int8: _native.KV_INT8}
 
 
@@ -136,21 +133,28 @@ def _check_lens(t, name: str, B: int, dev) -> int:
     return t.data_ptr()
 
 
-def _on(dev: torch.device):
-    """Makes ``dev`` the current device for the calls inside (nothing to do where it is)."""
-    return nullcontext() if torch.cuda.current_device() == dev.index else torch.cuda.device(dev)
+def _call(what: str, fn, dev: torch.device, *args) -> None:
+    """``fn(*args, stream)`` with ``dev`` current and its current stream.
 
-
-def _stream(dev: torch.device) -> int:
-    """The current stream's handle (without the Stream object that ``torch.cuda.current_stream`` makes)."""
-    return torch._C._cuda_getCurrentRawStream(dev.index)
+    The raw handles are read without the device guard and the Stream object of
+    ``torch.cuda``: together some 3 us of a call that takes 14 to 25 on the host.
+    """
+    index = dev.index
+    if torch._C._cuda_getDevice() == index:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        _native.check(rc, what)
 
 
 @lru_cache(maxsize=256)
 def _decode_workspace_bytes(B: int, Smax: int, Hq: int, Hkv: int, weights: bool, device_index: int) -> int:
-    """The decode step's workspace on the current device, ``device_index``: a function of the shapes."""
+    """The decode step's workspace on a device: a function of the shapes."""
     lib = _native.load()
-    nbytes = int(lib.swa_kv_decode_workspace_bytes(B, Smax, Hq, Hkv, int(weights)))
+    with torch.cuda.device(device_index):
+        nbytes = int(lib.swa_kv_decode_workspace_bytes(B, Smax, Hq, Hkv, int(weights)))
     if nbytes <= 0:
         raise RuntimeError("decode workspace size query failed: " + lib.swa_last_error_string().decode(errors="replace"))
     return nbytes
@@ -179,23 +183,18 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     token = k_new.ndim == 3
     T = 1 if token else int(k_new.shape[1])
     shape = (B, Hkv, HEAD_DIM) if token else (B, T, Hkv, HEAD_DIM)
-    strides = []
-    for t, name in ((k_new, "k_new"), (v_new, "v_new")):
-        st = _check_rows(t, name, shape, dev)
-        strides.append(_Strides(st[0], 0, st[1]) if token else _Strides(st[0], st[1], st[2]))
+    ks, vs = _check_rows(k_new, "k_new", shape, dev), _check_rows(v_new, "v_new", shape, dev)
     lens_ptr = None if new_lens is None else _check_lens(new_lens, "new_lens", B, dev)
     seq_ptr = cache.seq_lens.data_ptr()
     start_ptr = seq_ptr if start is None else _check_lens(start, "start", B, dev)
     if T == 0:
         return
     weights = cache.key_weights
-    with _on(dev):
-        rc = _native.load().swa_kv_append(
-            k_new.data_ptr(), v_new.data_ptr(), strides[0], strides[1], start_ptr, lens_ptr, cache.k.data_ptr(),
-            cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
-            None if weights is None else weights.data_ptr(), seq_ptr, B, T, Hkv, Smax, HEAD_DIM, cache.block_size,
-            _DTYPES[cache.k.dtype], _stream(dev))
-    _native.check(rc, "switch_kv_cache_append")
+    _call("switch_kv_cache_append", _native.load().swa_kv_append, dev, k_new.data_ptr(), v_new.data_ptr(),
+          ks[0], 0 if token else ks[1], ks[-2], vs[0], 0 if token else vs[1], vs[-2], start_ptr, lens_ptr,
+          cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(),
+          None if weights is None else weights.data_ptr(), seq_ptr, B, T, Hkv, Smax, HEAD_DIM, cache.block_size,
+          _DTYPES[cache.k.dtype])
 
 
 def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: torch.Tensor, *,
@@ -238,16 +237,14 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
     weights = cache.key_weights if accumulate else None
     out = q.new_empty((B, Hq, HEAD_DIM))
     lse = cache.k_scale.new_empty((B, Hq))
-    with _on(dev):
-        nbytes = _decode_workspace_bytes(B, Smax, Hq, Hkv, weights is not None, dev.index)
-        ws = cache.seq_lens.new_empty((nbytes + 15) // 16 * 4)
-        route = route_full if route_full.is_contiguous() else route_full.contiguous()
-        rc = _native.load().swa_kv_decode(
-            q.data_ptr(), st[0], st[1], cache.k.data_ptr(), cache.v.data_ptr(), cache.k_scale.data_ptr(),
-            cache.v_scale.data_ptr(), cache.seq_lens.data_ptr(), route.data_ptr(), out.data_ptr(), lse.data_ptr(),
-            None if weights is None else weights.data_ptr(), B, Smax, Hq, Hkv, HEAD_DIM, cache.block_size,
-            min(int(window_size), Smax), float(scale), _DTYPES[cache.k.dtype], ws.data_ptr(), nbytes, _stream(dev))
-    _native.check(rc, "switch_gqa_decode_cached")
+    nbytes = _decode_workspace_bytes(B, Smax, Hq, Hkv, weights is not None, dev.index)
+    ws = cache.seq_lens.new_empty((nbytes + 15) // 16 * 4)
+    route = route_full if route_full.is_contiguous() else route_full.contiguous()
+    _call("switch_gqa_decode_cached", _native.load().swa_kv_decode, dev, q.data_ptr(), st[0], st[1], cache.k.data_ptr(),
+          cache.v.data_ptr(), cache.k_scale.data_ptr(), cache.v_scale.data_ptr(), cache.seq_lens.data_ptr(),
+          route.data_ptr(), out.data_ptr(), lse.data_ptr(), None if weights is None else weights.data_ptr(), B, Smax,
+          Hq, Hkv, HEAD_DIM, cache.block_size, min(int(window_size), Smax), float(scale), _DTYPES[cache.k.dtype],
+          ws.data_ptr(), nbytes)
     if status_out is not None or _core.CHECK_DEVICE_STATUS:
         _core.publish_status(ws[0:1], status_out)
     if squeeze:
@@ -280,7 +277,7 @@ def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, rec
     if keep >= Smax:  # no sequence is longer
         keep, sink, recent = Smax, 0, 0
     src = _pointers(cache)
-    dst, So = src, Smax
+    dst, So = src, Smax  # in place
     if out is not None and out is not cache:
         Bo, Ho, So, dev_out = _check_cache(out, "out")
         if (Bo, Ho) != (B, Hkv) or out.k.dtype != cache.k.dtype or out.block_size != cache.block_size:
@@ -293,15 +290,14 @@ def switch_kv_cache_evict(cache: SwitchKVCache, *, keep: int, sink: int = 0, rec
             raise ValueError("out holds fewer rows than are kept")
         dst = _pointers(out)
         ends = [0, 0]  # of the cache's and of out's memory up to here, by address
-        for first, end, owner in sorted(_spans(cache, src, 0) + _spans(out, dst, 1)):
+        for first, end, owner in sorted(_spans(src, B, Hkv, Smax, cache.block_size, 0) +
+                                        _spans(dst, B, Hkv, So, cache.block_size, 1)):
             if first < ends[1 - owner]:
                 raise ValueError("out must not share memory with the cache")
             ends[owner] = max(ends[owner], end)
     slots = cache.seq_lens.new_empty((B, Hkv, keep))
-    with _on(dev):
-        rc = _native.load().swa_kv_evict(*src, *dst, slots.data_ptr(), B, Hkv, Smax, So, HEAD_DIM, cache.block_size,
-                                         keep, sink, recent, _DTYPES[cache.k.dtype], _stream(dev))
-    _native.check(rc, "switch_kv_cache_evict")
+    _call("switch_kv_cache_evict", _native.load().swa_kv_evict, dev, *src, *dst, slots.data_ptr(), B, Hkv, Smax, So,
+          HEAD_DIM, cache.block_size, keep, sink, recent, _DTYPES[cache.k.dtype])
     return slots
 
 
@@ -310,8 +306,10 @@ def _pointers(c: SwitchKVCache) -> tuple:
             c.seq_lens.data_ptr())
 
 
-def _spans(c: SwitchKVCache, ptrs: tuple, owner: int) -> list:
-    """``(first byte, end, owner)`` of the cache's tensors."""
-    rows, scales = c.k.numel(), 4 * c.k_scale.numel()
-    sizes = (rows, rows, scales, scales, 4 * c.key_weights.numel(), 4 * c.seq_lens.numel())
-    return [(p, p + n, owner) for p, n in zip(ptrs, sizes)]
+def _spans(ptrs: tuple, B: int, Hkv: int, Smax: int, block: int, owner: int) -> list:
+    """``(first byte, end, owner)`` of a cache's tensors."""
+    k, v, ks, vs, w, n = ptrs
+    weights = 4 * B * Hkv * Smax
+    rows, scales = HEAD_DIM // 4 * weights, 4 * B * Hkv * -(-Smax // block)
+    return [(k, k + rows, owner), (v, v + rows, owner), (ks, ks + scales, owner), (vs, vs + scales, owner),
+            (w, w + weights, owner), (n, n + 4 * B, owner)]

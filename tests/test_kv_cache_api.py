@@ -125,13 +125,11 @@ def test_evict_refusals():
 def test_c_abi_refusals():
     # refused before any device call: the library needs no GPU for these
     lib = _native.load()
-    st = (ctypes.c_int64 * 3)(256, 256, 128)
-    odd = (ctypes.c_int64 * 3)(256, 256, 4)
     one, two, three, four = (ctypes.c_void_p(x) for x in (256, 512, 768, 1024))
     none = None
 
-    def append(k=one, v=one, ks=st, B=1, T=1, H=1, S=16, D=128, block=16, dtype=1, start=one, new=none, vc=two, vs=four, lens=one):
-        return lib.swa_kv_append(k, v, ks, st, start, new, one, vc, three, vs, none, lens, B, T, H, S, D, block, dtype, none)
+    def append(k=one, v=one, ks=128, B=1, T=1, H=1, S=16, D=128, block=16, dtype=1, start=one, new=none, vc=two, vs=four, lens=one):
+        return lib.swa_kv_append(k, v, 256, 256, ks, 256, 256, 128, start, new, one, vc, three, vs, none, lens, B, T, H, S, D, block, dtype, none)
 
     def decode(q=one, sb=128, B=1, S=16, Hq=2, H=1, D=128, block=16, window=4, scale=1.0, dtype=1, ws=one, nbytes=0):
         return lib.swa_kv_decode(q, sb, 128, one, one, one, one, one, one, one, one, none, B, S, Hq, H, D, block, window, scale,
@@ -142,7 +140,7 @@ def test_c_abi_refusals():
                                 recent, dtype, none)
 
     invalid, unsupported = -1, -3
-    for rc in (append(k=none), append(start=none), append(lens=none), append(k=ctypes.c_void_p(8)), append(ks=odd), append(ks=none),
+    for rc in (append(k=none), append(start=none), append(lens=none), append(k=ctypes.c_void_p(8)), append(ks=4), append(ks=-4),
                append(B=0), append(T=0), append(H=-1), append(S=0), append(block=48), append(dtype=0), decode(q=none),
                decode(q=ctypes.c_void_p(4)), decode(sb=4), decode(B=0), decode(Hq=3, H=2), decode(Hq=0), decode(window=0),
                decode(scale=0.0), decode(scale=math.nan), decode(block=8), decode(dtype=3), decode(ws=none), evict(k=none),
