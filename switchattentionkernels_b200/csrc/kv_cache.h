@@ -74,21 +74,25 @@ cudaError_t launch_kv_evict(const KvEvictParams& p, bool int8, bool in_place, in
 
 // Decode over the cache.  The (sequence, KV head, head block) units' legal keys are
 // cut into tiles of 128 keys.  All units of the batch are laid end to end along one axis
-// of work, in the order (sequence, KV head, head block), each as `omega` steps for
+// of work, in the order (head block, sequence, KV head), each as `omega` steps for
 // starting it and kTileSteps for every tile, and the axis is cut into equal shares, one
-// a CTA: a tile belongs to the CTA on whose share its first step lies.  A CTA's part of
-// one unit is a segment; its partial result lies in slot unit + cta (both grow along the
-// axis and each new segment moves one of them, so slots are distinct).
+// a CTA: a tile belongs to the CTA on whose share its first step lies.  (The head blocks
+// are outermost so that the CTAs that read the same keys for different heads do so at
+// the same time, all but one of them from L2.)  A CTA's part of one unit is a segment; its
+// partial result lies in slot unit + cta (both grow along the axis and each new segment
+// moves one of them, so slots are distinct).
 constexpr int kTileSteps = 2;
 
 // What CTA c's share begins with, and the whole plan.
 struct __align__(16) KvShare {
-  int b, u, off, left;    // sequence, unit in it, first step in the unit, steps of the share
-  int vbase, tbase;       // steps and tiles of the batch before the unit
+  int hb, b, g;           // head block, sequence, KV head
+  int off, left;          // first step in the unit, steps of the share
+  int vbase, tbase;       // steps and tiles before the unit
   int lo, hi;             // legal keys of the sequence
   int omega;              // of the batch, as are
   int per, longer;        // steps of a share; the first `longer` shares have one more
-  int pad;
+  int block_steps, block_tiles;  // steps and tiles of one head block's units
+  int pad[2];
 };
 
 struct __align__(64) KvDecodeParams {

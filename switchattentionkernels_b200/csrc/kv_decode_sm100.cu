@@ -104,16 +104,17 @@ constexpr int kFewTiles = 4;
 
 // A CTA's share, segment by segment.
 struct Segments {
-  int b, u, off, left;  // of the next segment: sequence, unit in it (KV head x head block), first step in it; steps left
-  int vbase, tbase;     // steps and tiles of the batch before that unit
+  int hb, b, g, off, left;  // of the next segment: head block, sequence, KV head, first step in the unit; steps left
+  int vbase, tbase;     // steps and tiles before that unit
   int lo, hi, all;      // legal keys of sequence b, tiles of its units
   int omega;
   // the current segment
-  int cur_b, cur_u, cur_vbase, cur_tbase, cur_lo, cur_hi, cur_all, first, n;
+  int cur_hb, cur_b, cur_g, cur_vbase, cur_tbase, cur_lo, cur_hi, cur_all, first, n;
 
   __device__ __forceinline__ void start(const KvShare& s) {
+    hb = s.hb;
     b = s.b;
-    u = s.u;
+    g = s.g;
     off = s.off;
     left = s.left;
     vbase = s.vbase;
@@ -128,8 +129,9 @@ struct Segments {
     while (left > 0) {
       const int length = all > 0 ? omega + all * kTileSteps : 0;
       const int take = min(length - off, left);
+      cur_hb = hb;
       cur_b = b;
-      cur_u = u;
+      cur_g = g;
       cur_vbase = vbase;
       cur_tbase = tbase;
       cur_lo = lo;
@@ -143,9 +145,12 @@ struct Segments {
         off = 0;
         vbase += length;
         tbase += all;
-        if (all == 0 || ++u == p.Hkv * p.nhb) {  // (a sequence without a key has no unit)
-          u = 0;
-          ++b;
+        if (all == 0 || ++g == p.Hkv) {  // (a sequence without a key has no unit)
+          g = 0;
+          if (++b == p.B) {
+            b = 0;
+            ++hb;
+          }
           const KeyRange r = key_range(p, b);
           lo = r.lo;
           hi = r.hi;
@@ -247,7 +252,6 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
   KvShare* share = reinterpret_cast<KvShare*>(smem + Sm::misc + 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int cta = blockIdx.x;
-  const int units = p.Hkv * p.nhb;  // units of a sequence
 
   // set up what needs no global memory while the kernel before this one ends
   if (tid == 0) {
@@ -313,38 +317,42 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       if (w < warp) before += scan[w];
       total += scan[w];
     }
-    const int tiles = static_cast<int>(total & (kOne - 1)) * units;
-    const int omega = tiles >= kFewTiles * p.ctas ? kUnitSteps : 0;
-    auto steps_of = [&](int64_t x) {  // of x's sequences and tiles
-      return (static_cast<int>(x >> 32) * omega + static_cast<int>(x & (kOne - 1)) * kTileSteps) * units;
+    const int tiles = static_cast<int>(total & (kOne - 1)) * p.Hkv;  // of one head block
+    const int omega = tiles * p.nhb >= kFewTiles * p.ctas ? kUnitSteps : 0;
+    auto steps_of = [&](int64_t x) {  // of x's sequences and tiles, all KV heads
+      return (static_cast<int>(x >> 32) * omega + static_cast<int>(x & (kOne - 1)) * kTileSteps) * p.Hkv;
     };
-    const int steps = steps_of(total);
+    const int block_steps = steps_of(total), steps = block_steps * p.nhb;
     // every share holds the first step of a tile: they lie at most omega + kTileSteps apart
     const int ctas = max(1, min(p.ctas, steps / (omega + kTileSteps)));
     KvShare sh{};
     sh.omega = omega;
     sh.per = steps / ctas;
     sh.longer = steps % ctas;
+    sh.block_steps = block_steps;
+    sh.block_tiles = tiles;
     const int v0 = share_start(cta, sh.per, sh.longer), v1 = share_start(cta + 1, sh.per, sh.longer);
+    sh.hb = block_steps > 0 ? v0 / block_steps : 0;
+    const int w0 = v0 - sh.hb * block_steps;  // in its head block
     if (cta >= ctas || v0 >= v1) {
       if (tid == 0) {
         p.share[cta] = sh;
         *share = sh;
       }
-    } else if (v0 >= steps_of(before) && v0 < steps_of(before + sum)) {  // exactly one thread
+    } else if (w0 >= steps_of(before) && w0 < steps_of(before + sum)) {  // exactly one thread
       int64_t at = before;
       for (int b = b0;; ++b) {
         const int n = seq_tiles(p, b);
         const int64_t next = at + (n > 0 ? kOne + n : 0);
-        if (v0 < steps_of(next)) {
+        if (w0 < steps_of(next)) {
           const KeyRange kr = key_range(p, b);
-          const int length = omega + n * kTileSteps, in = v0 - steps_of(at);
+          const int length = omega + n * kTileSteps, in = w0 - steps_of(at);
           sh.b = b;
-          sh.u = in / length;
+          sh.g = in / length;
           sh.off = in % length;
           sh.left = v1 - v0;
           sh.vbase = v0 - sh.off;
-          sh.tbase = static_cast<int>(at & (kOne - 1)) * units + sh.u * n;
+          sh.tbase = sh.hb * tiles + static_cast<int>(at & (kOne - 1)) * p.Hkv + sh.g * n;
           sh.lo = kr.lo;
           sh.hi = kr.hi;
           break;
@@ -377,7 +385,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     int it = 0, iv = 0;  // K and V tiles issued
     bool ok = true;
     while (ok && seg.next(p)) {
-      const int row = seg.cur_b * p.Hkv + seg.cur_u / p.nhb;
+      const int row = seg.cur_b * p.Hkv + seg.cur_g;
       const float* scales = p.scale[lane >> 4] + static_cast<int64_t>(row) * p.nblk;
       for (int i = 0; i < seg.n; ++i) {
         const int s = it % kStages;
@@ -461,9 +469,9 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     int it = 0, nseg = 0;
     // Q of a segment: 16 threads per head, 8 dims each
     auto load_q = [&](const Segments& sg) {
-      const int h = tid >> 4, hb = sg.cur_u % p.nhb;
+      const int h = tid >> 4, hb = sg.cur_hb;
       if (h >= min(kHeads, p.r - hb * kHeads)) return make_uint4(0, 0, 0, 0);
-      const int head = (sg.cur_u / p.nhb) * p.r + hb * kHeads + h;
+      const int head = sg.cur_g * p.r + hb * kHeads + h;
       return *reinterpret_cast<const uint4*>(p.q + sg.cur_b * p.q_sb + head * p.q_sh + 8 * (tid & 15));
     };
     // its parts into shared memory, once the scores of the segment before are done
@@ -532,9 +540,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       seg = ahead;
       more = ahead.next(p);
       const uint4 q_next = more ? load_q(ahead) : make_uint4(0, 0, 0, 0);
-      const int g = seg.cur_u / p.nhb, hb = seg.cur_u % p.nhb;
-      const int head0 = g * p.r + hb * kHeads;           // first query head of the block
-      const int nh = min(kHeads, p.r - hb * kHeads);     // heads that exist
+      const int head0 = seg.cur_g * p.r + seg.cur_hb * kHeads;  // first query head of the block
+      const int nh = min(kHeads, p.r - seg.cur_hb * kHeads);    // heads that exist
       if (!(ok = warp_wait(q_full, nseg & 1, abort_flag))) break;
       float f[kHeads], m[kHeads], l[kHeads], o[kHeads], alpha[kHeads], beta[kHeads];
 #pragma unroll
@@ -677,7 +684,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       __syncwarp();
       if (lane == 0) mbar_arrive(l_full);
       if (!(ok = warp_wait(l_full, nseg & 1, abort_flag))) break;
-      const int64_t slot = static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + cta;
+      const int64_t slot = (static_cast<int64_t>(seg.cur_hb) * p.B + seg.cur_b) * p.Hkv + seg.cur_g + cta;
 #pragma unroll
       for (int h = 0; h < kHeads; ++h) {
         const float sum = (lb[h] + lb[8 + h]) + (lb[16 + h] + lb[24 + h]);
@@ -718,7 +725,6 @@ template <int kHeads, bool kWeights>
 __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_merge_kernel(const __grid_constant__ KvDecodeParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int c = blockIdx.x, y = blockIdx.y;
-  const int units = p.Hkv * p.nhb;
   cudaGridDependencySynchronize();
   const KvShare sh = p.share[c];
   Segments seg{};
@@ -742,12 +748,11 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
       }
     }
     if (!seg.next(p) || seg.first == 0 || seg.first + seg.n < seg.cur_all) return;
-    const int b = seg.cur_b, u = seg.cur_u;
-    const int hb = u % p.nhb;
+    const int b = seg.cur_b, hb = seg.cur_hb;
     if (h >= min(kHeads, p.r - hb * kHeads)) return;
     const int first = share_of(seg.cur_vbase + sh.omega, sh.per, sh.longer);
     const int nseg = c - first + 1;
-    const int64_t slot0 = static_cast<int64_t>(b) * units + u + first;
+    const int64_t slot0 = (static_cast<int64_t>(hb) * p.B + b) * p.Hkv + seg.cur_g + first;
     const float2* ml = reinterpret_cast<const float2*>(p.part_ml) + slot0 * kHeads + h;
     // 32 segments at a time, a lane each for their maxima and sums; their O rows are on the way meanwhile
     const float* po = p.part_o + (slot0 * kHeads + h) * 128 + tid;
@@ -776,7 +781,7 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
         }
       }
     }
-    const int64_t row = static_cast<int64_t>(b) * p.Hq + (u / p.nhb) * p.r + hb * kHeads + h;
+    const int64_t row = static_cast<int64_t>(b) * p.Hq + seg.cur_g * p.r + hb * kHeads + h;
     p.out[row * 128 + tid] = __float2bfloat16_rn(acc / L);
     if (tid == 0) p.lse[row] = lg2_approx(L) + M;
     return;
@@ -785,9 +790,9 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
     constexpr int kStep = kWeightBlocks * (kMergeThreads / 32);  // warps of the share
     int mine = y * (kMergeThreads / 32) + warp;                  // this warp's next tile, from the segment's first on
     while (seg.next(p)) {
-      const int g = seg.cur_u / p.nhb;
-      if (seg.cur_u % p.nhb != 0) continue;  // a key's tile of the first head block stands for the others' too
-      float* dst = p.weights + (static_cast<int64_t>(seg.cur_b) * p.Hkv + g) * p.Smax;
+      if (seg.cur_hb != 0) break;  // a key's tile of the first head block stands for the others' too
+      const int64_t unit = static_cast<int64_t>(seg.cur_b) * p.Hkv + seg.cur_g;
+      float* dst = p.weights + unit * p.Smax;
       float lse = 0.0f;  // of head lane % kHeads of head block `of`
       int of = -1;
       for (int i = mine; i < seg.n; i += kStep) {
@@ -797,7 +802,7 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
         for (int j = 0; j < 4; ++j) old[j] = key0 + 32 * j < seg.cur_hi ? dst[key0 + 32 * j] : 0.0f;
         for (int hb = 0; hb < p.nhb; ++hb) {
           const int nh = min(kHeads, p.r - hb * kHeads);
-          const float* sc = p.scores + static_cast<int64_t>(seg.cur_tbase + hb * seg.cur_all + seg.first + i) * kHeads * kTile + lane;
+          const float* sc = p.scores + static_cast<int64_t>(seg.cur_tbase + hb * sh.block_tiles + seg.first + i) * kHeads * kTile + lane;
           float s[kHeads][4];
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) {
@@ -806,11 +811,11 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
           }
           if (of != hb) {  // from the unit's segments, 32 / kHeads of them at a time
             of = hb;
-            const int v0 = seg.cur_vbase + sh.omega + hb * (sh.omega + seg.cur_all * kTileSteps);  // the unit's first tile
+            const int v0 = seg.cur_vbase + sh.omega + hb * sh.block_steps;  // the unit's first tile
             const int first = share_of(v0, sh.per, sh.longer);
             const int nseg = share_of(v0 + (seg.cur_all - 1) * kTileSteps, sh.per, sh.longer) - first + 1;
             const float2* ml = reinterpret_cast<const float2*>(p.part_ml) +
-                               (static_cast<int64_t>(seg.cur_b) * units + seg.cur_u + hb + first) * kHeads;
+                               (static_cast<int64_t>(hb) * p.B * p.Hkv + unit + first) * kHeads;
             float M = -INFINITY, L = 0.0f;
 #pragma unroll 4
             for (int k = lane; k < nseg * kHeads; k += 32) {
