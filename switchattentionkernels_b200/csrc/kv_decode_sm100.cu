@@ -75,6 +75,26 @@ __device__ __forceinline__ float warp_max(float x) {
   return y;
 }
 
+// x[h] over the warp's lanes for every head h, halving the heads with each of the first
+// steps (9 shuffles for 8 heads, 7 for 4, instead of 5 a head): lanes (32 / kHeads) h and on
+// return head h's.  x is overwritten.
+template <int kHeads, typename Op>
+__device__ __forceinline__ float reduce_heads(float* x, int lane, Op op) {
+  int d = 16;
+#pragma unroll
+  for (int k = kHeads / 2; k >= 1; k >>= 1, d >>= 1) {
+    const bool up = (lane & d) != 0;
+#pragma unroll
+    for (int j = 0; j < k; ++j) {
+      const float give = up ? x[j] : x[j + k];
+      x[j] = op(up ? x[j + k] : x[j], __shfl_xor_sync(0xffffffffu, give, d));
+    }
+  }
+#pragma unroll
+  for (; d >= 1; d >>= 1) x[0] = op(x[0], __shfl_xor_sync(0xffffffffu, x[0], d));
+  return x[0];
+}
+
 struct KeyRange {
   int lo, hi;
 };
@@ -585,23 +605,18 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         }
         // maxima of the tile over its keys
         float* rb = red + buf * 48;
-        float mt[kHeads], vref;
+        float mt[kHeads], vref = warp_max(vs);
 #pragma unroll
-        for (int h = 0; h < kHeads; ++h) mt[h] = warp_max(s[h]);
-        vref = warp_max(vs);
-        if (lane == 0) {
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) rb[warp * 12 + h] = mt[h];
-          rb[warp * 12 + kHeads] = vref;
-          mbar_arrive(&red_full[buf]);
-        }
+        for (int h = 0; h < kHeads; ++h) mt[h] = s[h];
+        const float top = reduce_heads<kHeads>(mt, lane, [](float a, float b) { return fmaxf(a, b); });
+        if (lane % (32 / kHeads) == 0) rb[warp * 12 + lane / (32 / kHeads)] = top;
+        if (lane == 1) rb[warp * 12 + kHeads] = vref;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&red_full[buf]);
         if (!(ok = warp_wait(&red_full[buf], (it >> 1) & 1, abort_flag))) break;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) mt[h] = fmaxf(mt[h], rb[w * 12 + h]);
-          vref = fmaxf(vref, rb[w * 12 + kHeads]);
-        }
+        for (int h = 0; h < kHeads; ++h) mt[h] = fmaxf(fmaxf(rb[h], rb[12 + h]), fmaxf(rb[24 + h], rb[36 + h]));
+        vref = fmaxf(fmaxf(rb[kHeads], rb[12 + kHeads]), fmaxf(rb[24 + kHeads], rb[36 + kHeads]));
         // P relative to the tile's maximum, V scales relative to the tile's largest
         const float vrel = vref > 0.0f ? vs / vref : 0.0f;
         float pr[kHeads], al[kHeads], be[kHeads];
@@ -665,22 +680,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
       if (!ok) break;
       // row sums over the keys (threads)
       float* lb = lred + (nseg & 1) * 32;
-      {
-        // over the warp, halving the heads with the first steps: lanes (32 / kHeads) h .. end with head h
-        int x = 16;
-#pragma unroll
-        for (int k = kHeads / 2; k >= 1; k >>= 1, x >>= 1) {
-          const bool up = (lane & x) != 0;
-#pragma unroll
-          for (int j = 0; j < k; ++j) {
-            const float give = up ? l[j] : l[j + k];
-            l[j] = (up ? l[j + k] : l[j]) + __shfl_xor_sync(0xffffffffu, give, x);
-          }
-        }
-#pragma unroll
-        for (; x >= 1; x >>= 1) l[0] += __shfl_xor_sync(0xffffffffu, l[0], x);
-        if (lane % (32 / kHeads) == 0) lb[warp * 8 + lane / (32 / kHeads)] = l[0];
-      }
+      const float lw = reduce_heads<kHeads>(l, lane, [](float a, float b) { return a + b; });
+      if (lane % (32 / kHeads) == 0) lb[warp * 8 + lane / (32 / kHeads)] = lw;
       __syncwarp();
       if (lane == 0) mbar_arrive(l_full);
       if (!(ok = warp_wait(l_full, nseg & 1, abort_flag))) break;
