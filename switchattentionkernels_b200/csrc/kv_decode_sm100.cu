@@ -613,22 +613,25 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         if (lane == 1) rb[warp * 12 + kHeads] = vref;
         __syncwarp();
         if (lane == 0) mbar_arrive(&red_full[buf]);
+        // (while the other warps' maxima come in: O of the tile before, whose product has been issued
+        // since that tile's P)
+        if (i > 0 && !(ok = take_o(it - 1))) break;
         if (!(ok = warp_wait(&red_full[buf], (it >> 1) & 1, abort_flag))) break;
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) mt[h] = fmaxf(fmaxf(rb[h], rb[12 + h]), fmaxf(rb[24 + h], rb[36 + h]));
         vref = fmaxf(fmaxf(rb[kHeads], rb[12 + kHeads]), fmaxf(rb[24 + kHeads], rb[36 + kHeads]));
         // P relative to the tile's maximum, V scales relative to the tile's largest
         const float vrel = vref > 0.0f ? vs / vref : 0.0f;
-        float pr[kHeads], al[kHeads], be[kHeads];
+        float pr[kHeads];
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
           const float mn = fmaxf(m[h], mt[h]);
-          al[h] = m[h] == -INFINITY ? 0.0f : ex2_approx(m[h] - mn);
-          be[h] = ex2_approx(mt[h] - mn);
+          alpha[h] = m[h] == -INFINITY ? 0.0f : ex2_approx(m[h] - mn);
+          const float be = ex2_approx(mt[h] - mn);
           m[h] = mn;
           const float e = ex2_approx(s[h] - mt[h]);
-          l[h] = fmaf(e, be[h], l[h] * al[h]);
-          be[h] *= vref * (kInt8 ? 1.0f / kInt8One : 1.0f / 256.0f);
+          l[h] = fmaf(e, be, l[h] * alpha[h]);
+          beta[h] = be * (vref * (kInt8 ? 1.0f / kInt8One : 1.0f / 256.0f));
           pr[h] = e * vrel;
         }
         uint8_t* pb = smem + Sm::p + buf * kCols * 128;
@@ -669,12 +672,6 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         fence_proxy_async_smem();
         tc_fence_before();
         mbar_arrive(&p_full[buf]);
-        if (i > 0 && !(ok = take_o(it - 1))) break;
-#pragma unroll
-        for (int h = 0; h < kHeads; ++h) {
-          alpha[h] = al[h];
-          beta[h] = be[h];
-        }
       }
       if (ok) ok = take_o(it - 1);
       if (!ok) break;
