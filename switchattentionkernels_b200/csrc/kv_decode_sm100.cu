@@ -21,13 +21,15 @@
 // maximum (never above 1) and V relative to the tile's largest V scale.
 //
 // Measured (B200, graph of ten calls): 64 sequences of 16K-32K keys, an eighth routed full, 359 MB
-// of legal bytes, 64 to 68 us (5.3 to 5.6 TB/s; the e4m3 cache with one scale per head, whose bytes are
+// of legal bytes, 61 to 65 us (5.5 to 5.9 TB/s; the e4m3 cache with one scale per head, whose bytes are
 // converted in registers, takes 154 us); 536 MB of full sequences 85 us (6.3 TB/s).  Reading alone,
 // tiles of this size stream at 7.1 TB/s with 96 to 128 KB in flight per SM and at 6.5 to 7.0 with
 // 192 KB; two CTAs an SM with two K and two V tiles each hold 128 KB (three tiles each: 75.2
 // against 73.5 us on the 64 sequences; three CTAs: 81 us, their registers spill).  The
 // tensor pipe is 8 % busy.  What is left is the start (about 4 us to the first scores), the
-// uneven end and the second kernel (about 3 us).
+// uneven end and the second kernel (about 3 us).  With more than 8 query heads per KV head every
+// tile is taken once per 8 heads, and the softmax warps' chain per tile (about 2400 cycles)
+// bounds: 8 x 32K keys, 16 heads per KV head, 80 us for 41 us of bytes.
 #include <cuda_fp16.h>
 
 #include "kv_cache.h"
