@@ -48,7 +48,7 @@ constexpr int kScaleRing = 8;              // tiles whose block scales are held
 constexpr int kThreads = 192;
 constexpr int kParts = 3;
 constexpr float kE4m3Step = 16.0f;         // weight of an e4m3 part against the next
-constexpr float kInt8One = 8323072.0f;     // 127 * 65536: 1.0 as three signed-byte digits
+constexpr float kInt8One = 127.0f * 65536.0f;  // 1.0 as three signed-byte digits
 
 template <int kHeads>
 struct KvSmem {
@@ -216,7 +216,7 @@ __device__ __forceinline__ void split_e4m3(__half2 x, uint16_t* part) {
   part[2] = f16x2_to_e4m3x2(*reinterpret_cast<uint32_t*>(&y));
 }
 
-// A value in [-1, 1] in steps of 1 / 8323072 as three signed bytes (byte 2 the highest).
+// A value in [-1, 1] in steps of 1 / (127 * 65536) as three signed bytes (byte 2 the highest).
 __device__ __forceinline__ uint32_t split_int8(float x) {
   return static_cast<uint32_t>(__float2int_rn(x * kInt8One) + 0x008080) ^ 0x008080u;
 }

@@ -112,7 +112,7 @@ def decode(c: dict, q, route, window: int, sm_scale=None):
             eW[b, g, lo:L] = (w * rel).sum(0)
             # O: P to FP16 (2^-11) and FP32 sums of 3 x 128 products (2^-14), on top of the weights'.
             # Then P's last step.  What is cut into three parts is x = 2^(s - m) vs / vref, m the largest
-            # score and vref the largest V scale of a tile: for int8 in steps of 1 / 8323072, so x is off
+            # score and vref the largest V scale of a tile: for int8 in steps of 1 / (127 * 65536), so x is off
             # by at most 1 / 16646144 < 2^-23.9 and the key's share of O by that times 2^(m - lse) vref
             # |v8| <= 2^-23.9 max(vs) |v8|; for e4m3 (steps of 2^-17 of 1 / 256, FP16's 2^-24 of it) by less.
             v8 = values(c["v"][b, g, lo:L]).abs()
