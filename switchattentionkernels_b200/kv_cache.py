@@ -122,7 +122,9 @@ def _check_rows(t, name: str, shape: tuple, dev) -> tuple:
     for s in st[:-1]:
         bits |= s
     if st[-1] != 1 or bits & 7:
-        raise ValueError(f"{name} needs contiguous, 16-byte aligned rows (other strides multiples of 8 elements)")
+        st = tuple(s if n > 1 else 0 for s, n in zip(st[:-1], shape)) + st[-1:]  # a single entry's stride is never used
+        if st[-1] != 1 or t.data_ptr() % 16 or any(s % 8 for s in st[:-1]):
+            raise ValueError(f"{name} needs contiguous, 16-byte aligned rows (other strides multiples of 8 elements)")
     return st
 
 

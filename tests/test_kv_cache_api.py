@@ -79,6 +79,13 @@ def test_append_refusals():
         for bad in (torch.zeros(2), torch.zeros(3, dtype=torch.int32), torch.zeros(2, 1, dtype=torch.int32), [1, 2]):
             with pytest.raises(ValueError, match=name):
                 switch_kv_cache_append(c, ok, ok, **{name: dev(bad) if isinstance(bad, torch.Tensor) else bad})
+    # the stride of a single entry does not matter, only its address
+    from switchattentionkernels_b200 import kv_cache
+    one = dev(torch.zeros(4096, dtype=torch.bfloat16).as_strided((1, 3, 1, 128), (37, 256, 5, 1)))
+    assert kv_cache._check_rows(one, "x", (1, 3, 1, 128), one.device) == (0, 256, 0, 1)
+    with pytest.raises(ValueError, match="multiples of 8"):
+        kv_cache._check_rows(dev(torch.zeros(4096, dtype=torch.bfloat16).as_strided((1, 3, 2, 128), (37, 256, 5, 1))), "x",
+                             (1, 3, 2, 128), one.device)
     empty = _rows(2, 0, 2, 128)
     switch_kv_cache_append(c, empty, empty)  # nothing to do: no launch
 
