@@ -173,19 +173,19 @@ __device__ __forceinline__ float grown_scale(uint32_t amax_bits, bool has_old, f
 // ---------------------------------------------------------------------------
 // append
 // ---------------------------------------------------------------------------
-// Rows that a CTA appends.
-__host__ __device__ constexpr int append_rows_of(int block) { return block < 64 ? 64 : block; }
+constexpr int kAppendRows = 128;  // rows that a CTA appends: one block or several
 
-// Chunks of many rows: one CTA per (64 rows, or one block of 128, KV head, K or V, sequence).  Each
+// Chunks of many rows: one CTA per (128 rows, KV head, K or V, sequence), whole blocks.  Each
 // thread keeps its part of the new rows in registers (16 bytes a pass of 16 rows), so the
 // rows are read once: maxima of the blocks, scales, rounding, store.  HBM-bound: 2 bytes read
-// and 1 written per value (4 x 16384 rows of 8 heads: 62 to 66 us for 61 us of copying; CTAs of a
-// single block took 121 us with blocks of 16 rows, 80 us with 32).
+// and 1 written per value (4 x 16384 rows of 8 heads: 60 us for 61 us of copying with blocks of
+// 64 or 128, 63 with 32, 74 with 16 (int8 84), whose maxima cross the warps eight times a CTA;
+// CTAs of 64 rows took 61, 67 and 76 us, CTAs of a single block 80 with 32 and 121 with 16).
 constexpr int kAppendThreads = 256;
 
 template <bool kInt8, int kBlock>
 __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_constant__ KvAppendParams p) {
-  constexpr int kRows = append_rows_of(kBlock);
+  constexpr int kRows = kAppendRows;
   constexpr int kPasses = kRows / 16;
   constexpr int kBlocks = kRows / kBlock;
   constexpr int kPer = kPasses / kBlocks;  // passes of a block
@@ -308,7 +308,7 @@ cudaError_t append_rows(const KvAppendParams& p, cudaStream_t stream) {
                                    : p.block == 32 ? kv_append_kernel<kInt8, 32>
                                    : p.block == 64 ? kv_append_kernel<kInt8, 64>
                                                    : kv_append_kernel<kInt8, 128>;
-  const dim3 grid((p.T - 1) / append_rows_of(p.block) + 2, 2 * p.Hkv, p.B);
+  const dim3 grid((p.T - 1) / kAppendRows + 2, 2 * p.Hkv, p.B);
   cudaError_t e = launch_dependent(kernel, grid, dim3(kAppendThreads), 0, stream, p);
   if (e != cudaSuccess || !p.lens_after) return e;
   return launch_dependent(kv_advance_kernel, dim3((p.B + 127) / 128), dim3(128), 0, stream, p);
