@@ -120,7 +120,7 @@ int swa_kv_append(const void* k_new, const void* v_new, int64_t k_stride_b, int6
   p.seq_lens = seq_lens;
   p.lens_after = start == seq_lens || new_lens == seq_lens;
   p.B = B;
-  p.T = T;
+  p.T = std::min(T, Smax);  // later rows are dropped wherever they start; row numbers stay below 2^31
   p.Hkv = Hkv;
   p.Smax = Smax;
   p.block = block_size;

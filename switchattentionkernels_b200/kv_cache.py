@@ -191,6 +191,7 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     start_ptr = seq_ptr if start is None else _check_lens(start, "start", B, dev)
     if T == 0:
         return
+    T = min(T, Smax)  # rows past Smax are dropped; an expanded view may have more than an int counts
     weights = cache.key_weights
     _call("switch_kv_cache_append", _native.load().swa_kv_append, dev, k_new.data_ptr(), v_new.data_ptr(),
           ks[0], 0 if token else ks[1], ks[-2], vs[0], 0 if token else vs[1], vs[-2], start_ptr, lens_ptr,

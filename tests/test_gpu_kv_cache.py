@@ -81,6 +81,26 @@ def test_append_matches_reference(cuda_device, dtype, B, T, Hkv, Smax, block):
         _equal(c, want)
 
 
+@pytest.mark.parametrize("Smax", [1, 100, 300])
+@pytest.mark.parametrize("T", [301, 2 ** 31 - 1, 2 ** 32 + 1])
+def test_append_more_rows_than_the_cache_has(cuda_device, T, Smax):
+    # one row expanded: behind the cached ones it fills the cache, whatever T and new_lens say
+    dev = cuda_device
+    g = torch.Generator().manual_seed(T % 1000 + Smax)
+    c = make_switch_kv_cache(2, Smax, 2, device=dev, block_size=16)
+    want = ref.clone(c)
+    first = _rows(g, 2, Smax, 2, 128)
+    lens = torch.tensor([0, Smax - 1], dtype=torch.int32)
+    switch_kv_cache_append(c, first.to(dev), first.to(dev), new_lens=lens.to(dev))
+    ref.append(want, first, first, lens)
+    k, v = _rows(g, 2, 1, 2, 128), _rows(g, 2, 1, 2, 128)
+    many = torch.full((2,), 2 ** 31 - 1, dtype=torch.int32, device=dev)
+    switch_kv_cache_append(c, k.to(dev).expand(2, T, 2, 128), v.to(dev).expand(2, T, 2, 128), new_lens=many)
+    ref.append(want, k.expand(2, Smax, 2, 128), v.expand(2, Smax, 2, 128), None)
+    torch.cuda.synchronize()
+    _equal(c, want)
+
+
 @BOTH
 def test_append_tokens_grow_a_block(cuda_device, dtype):
     # token by token, each larger than the last: the block's rows are rounded again at each doubling
