@@ -340,8 +340,8 @@ int swa_prefill_forward_noalloc(const void* q, const void* k, const void* v, con
  * becomes the smallest power of two (at least 2^-126; 0 for a block of zeros) that both
  * its earlier rows' scale and the largest finite |value| of its new rows need (448 /
  * 127 times it reaches them); earlier rows of the block are rounded again when it
- * differs from what it was.  Values are rounded to nearest even; infinities saturate,
- * NaN stays NaN (e4m3) or becomes 0 (int8).  key_weights (nullable): new rows start at 0. */
+ * differs from what it was.  Values are rounded to nearest even; infinities saturate
+ * (0 under a scale of 0), NaN stays NaN (e4m3) or becomes 0 (int8).  key_weights (nullable): new rows start at 0. */
 int swa_kv_append(const void* k_new, const void* v_new, int64_t k_stride_b, int64_t k_stride_t, int64_t k_stride_h,
                   int64_t v_stride_b, int64_t v_stride_t, int64_t v_stride_h, const int32_t* start, const int32_t* new_lens, void* k_cache, void* v_cache, float* k_scale,
                   float* v_scale, float* key_weights, int32_t* seq_lens, int B, int T, int Hkv, int Smax,

@@ -176,8 +176,9 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
 
     A block's scale is the smallest power of two that its rows need, and only grows:
     when it does, the block's earlier rows are rounded again.  Rounding is to nearest
-    even; infinities saturate and do not count for the scale, NaN stays NaN in an e4m3
-    cache and becomes 0 in an int8 one.  Appended rows start with ``key_weights`` 0.
+    even; infinities saturate and do not count for the scale (0 in a block without another
+    value but zeros), NaN stays NaN in an e4m3 cache and becomes 0 in an int8 one.
+    Appended rows start with ``key_weights`` 0.
     """
     B, Hkv, Smax, dev = _check_cache(cache)
     if not isinstance(k_new, torch.Tensor) or k_new.ndim not in (3, 4):
