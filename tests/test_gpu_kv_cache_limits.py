@@ -45,3 +45,90 @@ def test_infinities_of_a_block_without_finite_values_are_zero(cuda_device, dtype
         v = (t.float() * s.repeat_interleave(32, 2)[..., None]).cpu()
         assert not v[:2, :, :T].any() and bool((v[:2, :, T:T + 2] == 1.0).all())
         assert torch.equal(torch.isnan(v[2]), nan)
+
+
+# --------------------------------------------------------------------------- decode
+def _within_its_own_size(c, q, route, W, label):
+    """Decode against 64 bits, the error counted against what each head's keys contribute."""
+    dev = c.k.device
+    before = ref.clone(c)
+    O, L = switch_gqa_decode_cached(q.to(dev), c, route.to(dev), window_size=W)
+    torch.cuda.synchronize()
+    want, lse, _, (_, eL, _) = ref.decode(before, q, route, W)
+    B, Hq, _ = q.shape
+    Hkv, bs = c.k.shape[1], c.block_size
+    r = Hq // Hkv
+    for b in range(B):
+        n = int(before["seq_lens"][b])
+        at = torch.arange(0 if bool(route[b]) else max(0, n - W), n)
+        for h in range(Hq):
+            g = h // r
+            k = ref.values(before["k"][b, g, at]) * ref.values(before["k_scale"][b, g])[at // bs][:, None]
+            vs = ref.values(before["v_scale"][b, g])[at // bs]
+            v8 = ref.values(before["v"][b, g, at]).abs()
+            qq = ref.values(q[b, h])
+            w = torch.exp2((k @ qq) * (ref.LOG2E / math.sqrt(128.0)) - lse[b, h])
+            # a weight: its score and the LSE, each a sum of 3 x 128 FP32 products times FP32 factors (off by at
+            # most (384 + 8) 2^-23 of the sum of magnitudes), exp2 and sums 2^-18; P rounded to FP16: 2^-11;
+            # the FP32 sums of 3 x 128 products again
+            ds = (k.abs() @ qq.abs()) * (ref.LOG2E / math.sqrt(128.0)) * (392 * 2.0 ** -23)
+            rel = math.log(2.0) * 1.01 * (ds + ds.max()) + 2.0 ** -18 + 2.0 ** -11 + 392 * 2.0 ** -23
+            # P's last step: 2^-24 (int8; e4m3 2^-26) of a reference that lies less than 2^4 above the
+            # largest w vs of its tile
+            last = 2.0 ** -20 * float((w * vs).max())
+            tol = (w * vs * rel) @ v8 + last * v8.sum(0)
+            tol = tol + (want[b, h].abs() + tol) * 2.0 ** -8  # and O to BF16
+            off = (O[b, h].cpu().double() - want[b, h]).abs()
+            i = int((off / tol.clamp(min=1e-300)).argmax())
+            assert bool((off <= tol).all()), f"{label}: head {h}, off by {off[i]:.3e} of {want[b, h, i]:.3e}, allowed {tol[i]:.3e}"
+    assert bool(((L.cpu().double() - lse).abs() <= eL).all()), label
+
+
+@BOTH
+@pytest.mark.parametrize("light,heavy", [(2.0 ** -20, 1.0), (2.0 ** -30, 1.0), (1.0, 2.0 ** 30), (3e-5, 7.0), (2.0 ** -60, 2.0 ** 60),
+                                         (2.0 ** -100, 2.0 ** -60), (0.25, 1.0), (1.0, 0.0)])
+@pytest.mark.parametrize("Hq,Hkv,block", [(2, 1, 16), (8, 1, 32), (12, 1, 64), (8, 2, 128)])
+def test_decode_v_scales_far_apart(cuda_device, dtype, light, heavy, Hq, Hkv, block):
+    # keys that take all of the weight lie under a V scale far below another block's of the same tile, whose
+    # keys take next to none, as much of the sum as the others, or all of it
+    dev = cuda_device
+    g = torch.Generator().manual_seed(Hq * 100 + block)
+    S, lens = 700, [700, 333, 130]
+    nb = -(-S // block)
+    is_heavy = torch.rand(3, Hkv, nb, generator=g) < 0.4
+    is_heavy[:, :, 0] = False
+    is_heavy[:, :, 1] = True
+    gap = math.log2(heavy / light) if heavy > 0 else 0.0
+    for below in (gap + 30.0, gap, 0.0):  # log2 of a light key's weight over a heavy one's
+        c = make_switch_kv_cache(3, S, Hkv, device=dev, dtype=dtype, block_size=block)
+        k = torch.randint(-2, 3, (3, Hkv, S, 128), generator=g).float()
+        # the first dim sets the score: 16 * d * 2^-3 log2(e) / sqrt(128) in log2 units
+        d = below / (16.0 * 2.0 ** -3 * ref.LOG2E / math.sqrt(128.0))
+        top = torch.where(is_heavy, -0.5 * d, 0.5 * d).clamp(-120.0, 120.0).round()
+        k[..., 0] = top.repeat_interleave(block, 2)[:, :, :S]
+        c.k.copy_(k.to(dtype).to(dev))
+        c.k_scale.fill_(2.0 ** -3)
+        c.v.copy_(torch.randint(-100, 101, (3, Hkv, S, 128), generator=g).float().to(dtype).to(dev))
+        c.v_scale.copy_(torch.where(is_heavy, torch.tensor(heavy), torch.tensor(light)).to(dev))
+        c.seq_lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        q = torch.randn(3, Hq, 128, generator=g).bfloat16()
+        q[..., 0] = 16.0
+        _within_its_own_size(c, q, torch.tensor([True, False, True]), 200, f"{light} {heavy} {below}")
+
+
+@BOTH
+@pytest.mark.parametrize("B,S,Hq,Hkv,block", [(24, 4000, 8, 4, 32), (6, 9000, 40, 2, 16)])
+def test_decode_v_scales_far_apart_in_some_tiles(cuda_device, dtype, B, S, Hq, Hkv, block):
+    # many tiles a CTA, every third stretch of 400 rows with scales of any size
+    dev = cuda_device
+    g = torch.Generator().manual_seed(S)
+    c = make_switch_kv_cache(B, S, Hkv, device=dev, dtype=dtype, block_size=block)
+    shape = (B, Hkv, c.k_scale.shape[2])
+    c.k.copy_(torch.randint(-100, 101, c.k.shape, generator=g).float().to(dtype).to(dev))
+    c.v.copy_(torch.randint(-100, 101, c.k.shape, generator=g).float().to(dtype).to(dev))
+    c.k_scale.copy_(2.0 ** torch.randint(-10, -5, shape, generator=g).float())
+    wild = torch.arange(shape[2]) * block // 400 % 3 == 1
+    c.v_scale.copy_(torch.where(wild, 2.0 ** torch.randint(-30, 1, shape, generator=g).float(), torch.tensor(2.0 ** -14)))
+    c.seq_lens.copy_(torch.randint(S // 2, S + 1, (B,), generator=g, dtype=torch.int32))
+    q = torch.randn(B, Hq, 128, generator=g).bfloat16()
+    _within_its_own_size(c, q, torch.rand(B, generator=g) < 0.5, 1000, f"B={B} S={S}")
