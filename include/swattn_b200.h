@@ -351,8 +351,8 @@ int swa_kv_append(const void* k_new, const void* v_new, int64_t k_stride_b, int6
  * q_stride_b + h * q_stride_h + d (multiples of 8).  key_weights (nullable): the
  * attention weight of each legal key, summed over the query heads of its group, is
  * added to it.  The workspace's first int32 is the status word (0 or
- * SWA_STATUS_TIMEOUT), valid once the call has run; the workspace needs no clearing
- * and calls that may overlap need one each. */
+ * SWA_STATUS_TIMEOUT: out and lse are undefined, key_weights unchanged), valid once the
+ * call has run; the workspace needs no clearing and calls that may overlap need one each. */
 size_t swa_kv_decode_workspace_bytes(int B, int Smax, int Hq, int Hkv, int with_weights);
 int swa_kv_decode(const void* q, int64_t q_stride_b, int64_t q_stride_h, const void* k_cache, const void* v_cache,
                   const float* k_scale, const float* v_scale, const int32_t* seq_lens, const uint8_t* route,

@@ -215,7 +215,8 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
 
     With ``accumulate`` and a cache that has ``key_weights``, the softmax weight of every
     row that was attended to, summed over the query heads of its KV head, is added to
-    them.  ``status_out``: as in ``switch_gqa_decode_forward``.
+    them.  ``status_out``: as in ``switch_gqa_decode_forward``; with a non-zero word
+    ``key_weights`` is unchanged.
     """
     B, Hkv, Smax, dev = _check_cache(cache)
     squeeze = isinstance(q, torch.Tensor) and q.ndim == 4

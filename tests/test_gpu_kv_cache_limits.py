@@ -132,3 +132,32 @@ def test_decode_v_scales_far_apart_in_some_tiles(cuda_device, dtype, B, S, Hq, H
     c.seq_lens.copy_(torch.randint(S // 2, S + 1, (B,), generator=g, dtype=torch.int32))
     q = torch.randn(B, Hq, 128, generator=g).bfloat16()
     _within_its_own_size(c, q, torch.rand(B, generator=g) < 0.5, 1000, f"B={B} S={S}")
+
+
+def test_decode_that_timed_out_leaves_the_weights(cuda_device):
+    # a withheld tile: the call reports it, key_weights are what they were, and the step can be taken again
+    from switchattentionkernels_b200 import _native
+    lib = _native.load()
+    dev = cuda_device
+    g = torch.Generator().manual_seed(61)
+    c = make_switch_kv_cache(64, 2000, 8, device=dev, block_size=64, track_weights=True)
+    x = torch.randn(64, 2000, 8, 128, generator=g).bfloat16().to(dev)
+    switch_kv_cache_append(c, x, x.flip(-1).contiguous())
+    c.key_weights.copy_(torch.rand(64, 8, 2000, generator=g))
+    before = c.key_weights.clone()
+    q = torch.randn(64, 32, 128, generator=g).bfloat16().to(dev)
+    route = torch.ones(64, dtype=torch.bool, device=dev)
+    O, L = switch_gqa_decode_cached(q, c, route)
+    after = c.key_weights.clone()
+    assert not torch.equal(after, before)
+    c.key_weights.copy_(before)
+    lib.swa_test_withhold_kv_load(1)
+    try:
+        with pytest.raises(RuntimeError, match="timed out"):
+            switch_gqa_decode_cached(q, c, route)
+    finally:
+        lib.swa_test_withhold_kv_load(0)
+    torch.cuda.synchronize()
+    assert torch.equal(c.key_weights, before)
+    again = switch_gqa_decode_cached(q, c, route)
+    assert torch.equal(again[0], O) and torch.equal(again[1], L) and torch.equal(c.key_weights, after)
