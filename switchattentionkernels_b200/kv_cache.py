@@ -170,8 +170,9 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     sequence; views with contiguous rows (slices of a fused projection) are taken as
     they are.  ``new_lens``: int32 ``[B]``, the rows of a padded batch that count (default:
     all ``T``).  ``start``: int32 ``[B]``, the row at which each sequence's new rows begin
-    (default ``cache.seq_lens``; earlier: the rows from there on are replaced, e.g. after
-    rejected draft tokens).  Neither may overlap ``cache.seq_lens`` unless it is that tensor.
+    (default ``cache.seq_lens``; earlier: the rows from there on are dropped and replaced, e.g.
+    after rejected draft tokens, also by no row at all; later: the rows between count as
+    cached and hold whatever lies there).  Neither may overlap ``cache.seq_lens`` unless it is that tensor.
     Rows that do not fit (``>= Smax``) are dropped.
 
     A block's scale is the smallest power of two that its rows need, and only grows:
@@ -190,7 +191,9 @@ def switch_kv_cache_append(cache: SwitchKVCache, k_new: torch.Tensor, v_new: tor
     lens_ptr = None if new_lens is None else _check_lens(new_lens, "new_lens", B, dev)
     seq_ptr = cache.seq_lens.data_ptr()
     start_ptr = seq_ptr if start is None else _check_lens(start, "start", B, dev)
-    if T == 0:
+    if T == 0:  # no new row: the sequences end at `start`
+        if start is not None:
+            torch.clamp(start, 0, Smax, out=cache.seq_lens)
         return
     T = min(T, Smax)  # rows past Smax are dropped; an expanded view may have more than an int counts
     weights = cache.key_weights

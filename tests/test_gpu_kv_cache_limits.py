@@ -47,6 +47,27 @@ def test_infinities_of_a_block_without_finite_values_are_zero(cuda_device, dtype
         assert torch.equal(torch.isnan(v[2]), nan)
 
 
+@BOTH
+def test_empty_batch_with_start_drops_the_rows_from_there_on(cuda_device, dtype):
+    # no new row (T = 0) is what new_lens = 0 is: the sequence ends at `start`
+    dev = cuda_device
+    g = torch.Generator().manual_seed(7)
+    x = torch.randn(3, 20, 2, 128, generator=g).bfloat16().to(dev)
+    start = torch.tensor([5, -3, 70], dtype=torch.int32, device=dev)
+    none = torch.zeros(3, dtype=torch.int32, device=dev)
+    got = []
+    for rows, lens in ((x[:, :0], None), (x[:, :0], none), (x, none), (x[:, :1], none)):
+        c = make_switch_kv_cache(3, 40, 2, device=dev, dtype=dtype, block_size=16, track_weights=True)
+        switch_kv_cache_append(c, x, x)
+        before = ref.clone(c)
+        switch_kv_cache_append(c, rows, rows, new_lens=lens, start=start)
+        got.append(c.seq_lens.tolist())
+        assert torch.equal(c.k.cpu().view(torch.uint8), before["k"].view(torch.uint8)) and torch.equal(c.k_scale.cpu(), before["k_scale"])
+    assert got == [[5, 0, 40]] * 4
+    switch_kv_cache_append(c, x[:, :0], x[:, :0])  # behind the cached rows: nothing changes
+    assert c.seq_lens.tolist() == [5, 0, 40]
+
+
 # --------------------------------------------------------------------------- decode
 def _within_its_own_size(c, q, route, W, label):
     """Decode against 64 bits, the error counted against what each head's keys contribute."""

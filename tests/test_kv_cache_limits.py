@@ -7,7 +7,8 @@ import pytest
 import torch
 
 import _kv_reference as ref
-from switchattentionkernels_b200 import make_switch_kv_cache
+from switchattentionkernels_b200 import SwitchKVCache, make_switch_kv_cache, switch_kv_cache_append
+from test_host_api import dev
 
 E4M3, INT8 = torch.float8_e4m3fn, torch.int8
 
@@ -28,3 +29,17 @@ def test_reference_infinities_saturate_at_the_scale(dtype):
     assert math.isnan(v[0, 2]) if dtype == E4M3 else v[0, 2] == 0.0
     top = ref.QMAX[dtype]
     assert v[16, :3].tolist() == [top, -top, 1.0 / float(s[1])]
+
+
+def test_empty_batch_ends_the_sequences_at_start():
+    c = make_switch_kv_cache(3, 40, 2, device="cpu", block_size=16)
+    c = SwitchKVCache(*(dev(t) for t in (c.k, c.v, c.k_scale, c.v_scale, c.seq_lens)), block_size=16)
+    c.seq_lens.fill_(20)
+    empty = dev(torch.zeros(3, 0, 2, 128, dtype=torch.bfloat16))
+    switch_kv_cache_append(c, empty, empty)
+    assert c.seq_lens.tolist() == [20, 20, 20]
+    lens = c.seq_lens
+    switch_kv_cache_append(c, empty, empty, start=dev(torch.tensor([5, -3, 70], dtype=torch.int32)))
+    assert lens.tolist() == [5, 0, 40] and c.seq_lens is lens
+    with pytest.raises(ValueError, match="start"):
+        switch_kv_cache_append(c, empty, empty, start=dev(torch.tensor([5, -3], dtype=torch.int32)))
