@@ -422,6 +422,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     const uint64_t once = l2_policy_evict_first();
     int it = 0, iv = 0;  // K and V tiles issued
     bool ok = true;
+    const int withheld = p.test_withhold != 0 && cta == 0 ? 1 : -1;  // K tile that is not loaded
     while (ok && seg.next(p)) {
       const int row = seg.cur_b * p.Hkv + seg.cur_g;
       const float* scales = p.scale[lane >> 4] + static_cast<int64_t>(row) * p.nblk;
@@ -430,7 +431,7 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
         const uint32_t ph = ((it / kStages) & 1) ^ 1;
         const int key0 = seg.cur_lo + (seg.first + i) * kTile;
         if (!(ok = warp_wait(&k_empty[s], ph, abort_flag))) break;
-        if (lane == 0 && !(p.test_withhold != 0 && cta == 0 && it == 1)) {
+        if (lane == 0 && it != withheld) {
           mbar_arrive_expect_tx(&k_full[s], kTileBytes);
           tma_load_3d_hint(smem + Sm::k + s * kTileBytes, &p.map[0], &k_full[s], 0, key0, row, once);
         }
@@ -452,7 +453,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
     if (*abort_flag && lane == 0) {
       // let the loads already issued land before the CTA's shared memory is released
       volatile int dummy = 0;
-      for (int t = max(0, it - kStages); t < it; ++t) mbar_wait(&k_full[t % kStages], (t / kStages) & 1, &dummy);
+      for (int t = max(0, it - kStages); t < it; ++t)
+        if (t != withheld) mbar_wait(&k_full[t % kStages], (t / kStages) & 1, &dummy);
       for (int t = max(0, iv - kStages); t < iv; ++t) mbar_wait(&v_full[t % kStages], (t / kStages) & 1, &dummy);
     }
   } else if (warp == 5) {

@@ -182,3 +182,25 @@ def test_decode_that_timed_out_leaves_the_weights(cuda_device):
     assert torch.equal(c.key_weights, before)
     again = switch_gqa_decode_cached(q, c, route)
     assert torch.equal(again[0], O) and torch.equal(again[1], L) and torch.equal(c.key_weights, after)
+
+
+def test_decode_that_times_out_takes_one_limit(cuda_device):
+    # the loads in flight are waited for before the CTA ends, the one that was never issued is not
+    from switchattentionkernels_b200 import _native
+    lib = _native.load()
+    c = make_switch_kv_cache(1, 300000, 1, device=cuda_device)
+    c.seq_lens.fill_(300000)
+    q = torch.zeros(1, 4, 128, dtype=torch.bfloat16, device=cuda_device)
+    route = torch.ones(1, dtype=torch.bool, device=cuda_device)
+    switch_gqa_decode_cached(q, c, route)
+    a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+    lib.swa_test_withhold_kv_load(1)
+    try:
+        a.record()
+        with pytest.raises(RuntimeError, match="timed out"):
+            switch_gqa_decode_cached(q, c, route)
+        b.record()
+    finally:
+        lib.swa_test_withhold_kv_load(0)
+    torch.cuda.synchronize()
+    assert 900 < a.elapsed_time(b) < 1800  # ms; a limit is 1 s
