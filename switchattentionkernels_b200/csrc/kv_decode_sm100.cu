@@ -35,6 +35,8 @@
 // uneven end and the second kernel (about 3 us).  With more than 8 query heads per KV head every
 // tile is taken once per 8 heads, and the softmax warps' chain per tile (about 2400 cycles)
 // bounds: 8 x 32K keys, 16 heads per KV head, 80 us for 41 us of bytes.
+#include <atomic>
+
 #include <cuda_fp16.h>
 
 #include "kv_cache.h"
@@ -918,15 +920,15 @@ __global__ void __launch_bounds__(kMergeThreads, kWeights ? 6 : 8) kv_decode_mer
 
 template <bool kInt8, int kHeads, bool kWeights>
 cudaError_t launch_main(const KvDecodeParams& p, cudaStream_t stream) {
-  static bool attr_set[64] = {};
+  static std::atomic<bool> attr_set[64];  // host threads may call at once; setting it twice does no harm
   int dev = 0;
   cudaError_t e = cudaGetDevice(&dev);
   if (e != cudaSuccess) return e;
-  if (dev >= 64 || !attr_set[dev]) {
+  if (dev >= 64 || !attr_set[dev].load(std::memory_order_acquire)) {
     e = cudaFuncSetAttribute(kv_decode_kernel<kInt8, kHeads, kWeights>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                              KvSmem<kHeads>::bytes);
     if (e != cudaSuccess) return e;
-    if (dev < 64) attr_set[dev] = true;
+    if (dev < 64) attr_set[dev].store(true, std::memory_order_release);
   }
   e = launch_dependent(kv_decode_kernel<kInt8, kHeads, kWeights>, dim3(p.ctas), dim3(kThreads), KvSmem<kHeads>::bytes, stream, p);
   if (e != cudaSuccess) return e;

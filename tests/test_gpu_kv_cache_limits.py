@@ -204,3 +204,41 @@ def test_decode_that_times_out_takes_one_limit(cuda_device):
         lib.swa_test_withhold_kv_load(0)
     torch.cuda.synchronize()
     assert 900 < a.elapsed_time(b) < 1800  # ms; a limit is 1 s
+
+
+def test_first_calls_from_several_threads(cuda_device):
+    # every thread with its own cache and stream; the results are those of the calls one by one
+    import threading
+    dev = cuda_device
+    g = torch.Generator().manual_seed(67)
+    jobs = []
+    for i in range(6):
+        c = make_switch_kv_cache(2, 3000, 2, device=dev, dtype=(E4M3, INT8)[i % 2], block_size=64, track_weights=i % 3 == 0)
+        x = torch.randn(2, 2500, 2, 128, generator=g).bfloat16().to(dev)
+        q = torch.randn(2, (8, 16)[i // 3], 128, generator=g).bfloat16().to(dev)
+        jobs.append((c, x, q, torch.cuda.Stream()))
+    route = torch.tensor([True, False], device=dev)
+    torch.cuda.synchronize()
+    got, errors = [None] * 6, []
+
+    def work(i):
+        c, x, q, stream = jobs[i]
+        try:
+            with torch.cuda.stream(stream):
+                switch_kv_cache_append(c, x, x)
+                got[i] = [switch_gqa_decode_cached(q, c, route, accumulate=False) for _ in range(5)]
+                stream.synchronize()
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert not errors
+    for i, (c, _, q, _) in enumerate(jobs):
+        O, L = switch_gqa_decode_cached(q, c, route, accumulate=False)
+        assert c.seq_lens.tolist() == [2500, 2500]
+        for o, lse in got[i]:
+            assert torch.equal(o, O) and torch.equal(lse, L)
