@@ -112,28 +112,18 @@ __device__ __forceinline__ uint32_t abs_max_bits(const uint4* v, bool& finite) {
   return m;
 }
 
-// Packed BF16 values with zeros for infinities: what an infinity is under the scale 0 of a
-// block that holds no finite value but zeros (it saturates at 448 or 127 times the scale).
-// Times 0 it would be the NaN that only a NaN may become.
-__device__ __forceinline__ uint32_t inf_to_zero(uint32_t pair) {
-  if ((pair & 0x7FFFu) == 0x7F80u) pair &= ~0x7FFFu;
-  if ((pair & 0x7FFF0000u) == 0x7F800000u) pair &= ~0x7FFF0000u;
-  return pair;
-}
-
 __device__ __forceinline__ float bf_lo(uint32_t pair) { return __uint_as_float(pair << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t pair) { return __uint_as_float(pair & 0xFFFF0000u); }
 
 // Eight BF16 values times `inv` (a power of two that brings finite ones within 127 /
 // 448) to 8 bits.  The append is bound by instructions before it is by HBM, so:
 //   e4m3: the product in packed BF16, which is exact (a result too small for BF16's
-//   normal range is far below half of e4m3's smallest step); under the scale 0 (inv 0)
-//   infinities become zeros first;
+//   normal range is far below half of e4m3's smallest step);
 //   int8: x inv + 1.5 * 2^23 in one FMA, whose low byte is x inv rounded to nearest even
 //   (the sum's unit in the last place is 1); infinities and NaN go the long way.
 template <bool kInt8>
 __device__ __forceinline__ uint2 quantize8(uint4 v, float inv, bool finite) {
-  uint32_t w[4] = {v.x, v.y, v.z, v.w};
+  const uint32_t w[4] = {v.x, v.y, v.z, v.w};
   uint32_t o[2];
   if constexpr (kInt8) {
     if (finite) {
@@ -150,10 +140,6 @@ __device__ __forceinline__ uint2 quantize8(uint4 v, float inv, bool finite) {
         o[h] = pack8<true>(bf_lo(w[2 * h]) * inv, bf_hi(w[2 * h]) * inv, bf_lo(w[2 * h + 1]) * inv, bf_hi(w[2 * h + 1]) * inv);
     }
   } else {
-    if (!finite && inv == 0.0f) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) w[i] = inf_to_zero(w[i]);
-    }
     const __nv_bfloat162 f = __float2bfloat162_rn(inv);
     uint32_t y[4];
 #pragma unroll
@@ -182,6 +168,15 @@ template <bool kInt8>
 __device__ __forceinline__ float grown_scale(uint32_t amax_bits, bool has_old, float old_scale) {
   const float need = scale_for<kInt8>(__uint_as_float(amax_bits << 16));
   return has_old ? fmaxf(pow2_at_least(old_scale, 0, 0u), need) : need;
+}
+
+// What a block's values are multiplied by (a power of two: exact).  A block with the scale 0 holds
+// zeros, infinities and NaN.  e4m3: they are rounded as they are, so that infinities saturate
+// (their value, 448 times the scale, is 0) and only NaN becomes NaN; infinity times 0 would be one
+// too.  int8: times 0, where all of them become 0.
+template <bool kInt8>
+__device__ __forceinline__ float inverse_scale(float s) {
+  return s > 0.0f ? 1.0f / s : (kInt8 ? 0.0f : 1.0f);
 }
 
 // ---------------------------------------------------------------------------
@@ -245,7 +240,7 @@ __global__ void __launch_bounds__(kAppendThreads) kv_append_kernel(const __grid_
     const uint32_t amax = __reduce_max_sync(0xffffffffu, warp_max[j][tid & (kWarps - 1)]);
     const bool has_old = any_old && j == old_block;
     const float s = grown_scale<kInt8>(amax, has_old, old_scale);
-    const float inv = s > 0.0f ? 1.0f / s : 0.0f;  // a power of two: exact
+    const float inv = inverse_scale<kInt8>(s);
     if (has_old && s != old_scale) {
       const float ratio = old_scale / s;
       for (int i = tid; i < (rg.start - block0) * 8; i += kAppendThreads) {
@@ -290,12 +285,12 @@ __global__ void __launch_bounds__(1024) kv_append_token_kernel(const __grid_cons
       const int64_t unit = static_cast<int64_t>(b) * p.Hkv + g;
       uint8_t* cache = p.cache[kv] + unit * p.Smax * 128;
       float* scale = p.scale[kv] + unit * p.nblk + blk;
-      uint2 v = *reinterpret_cast<const uint2*>(p.x[kv] + b * p.sb[kv] + g * p.sh[kv] + 4 * lane);
+      const uint2 v = *reinterpret_cast<const uint2*>(p.x[kv] + b * p.sb[kv] + g * p.sh[kv] + 4 * lane);
       const float old_scale = *scale;
       const uint32_t amax = __reduce_max_sync(0xffffffffu, max(finite_abs_max(v.x), finite_abs_max(v.y)));
       const bool has_old = rg.start > row0;
       const float s = grown_scale<kInt8>(amax, has_old, old_scale);
-      const float inv = s > 0.0f ? 1.0f / s : 0.0f;
+      const float inv = inverse_scale<kInt8>(s);
       if (has_old && s != old_scale) {
         const float ratio = old_scale / s;
         for (int i = lane; i < (rg.start - row0) * 8; i += 32) {
@@ -303,7 +298,6 @@ __global__ void __launch_bounds__(1024) kv_append_token_kernel(const __grid_cons
           *q = rescale8<kInt8>(*q, ratio);
         }
       }
-      if (s == 0.0f) v = make_uint2(inf_to_zero(v.x), inf_to_zero(v.y));
       reinterpret_cast<uint32_t*>(cache + static_cast<int64_t>(rg.start) * 128)[lane] =
           pack8<kInt8>(bf_lo(v.x) * inv, bf_hi(v.x) * inv, bf_lo(v.y) * inv, bf_hi(v.y) * inv);
       __syncwarp();

@@ -66,7 +66,7 @@ def append(c: dict, k_new, v_new, new_lens=None, start=None) -> None:
                     if lo > blk * bs and new != old:
                         past = values(cache[b, g, blk * bs:lo])
                         cache[b, g, blk * bs:lo] = round8(past * (old / new), dtype)
-                    cache[b, g, lo:hi] = round8(rows / new if new > 0 else rows.clamp(-1.0, 1.0) * 0.0, dtype)
+                    cache[b, g, lo:hi] = round8(rows / new if new > 0 else rows * (dtype != torch.int8), dtype)
                     scale[b, g, blk] = new
         if c["key_weights"] is not None:
             c["key_weights"][b, :, s0:e0] = 0.0

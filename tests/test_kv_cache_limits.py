@@ -23,12 +23,12 @@ def test_reference_infinities_saturate_at_the_scale(dtype):
     c = ref.clone(make_switch_kv_cache(1, 32, 1, device="cpu", dtype=dtype, block_size=16))
     ref.append(c, x, x)
     s = c["k_scale"][0, 0]
-    v = ref.values(c["k"])[0, 0]
+    v = ref.values(c["k"])[0, 0] * s.double().repeat_interleave(16)[:, None]
     assert s.tolist() == [0.0, 2.0 ** -8 if dtype == E4M3 else 2.0 ** -6]
     assert v[0, :2].tolist() == [0.0, 0.0] and not v[1:16].any() and not v[0, 3:].any()
     assert math.isnan(v[0, 2]) if dtype == E4M3 else v[0, 2] == 0.0
     top = ref.QMAX[dtype]
-    assert v[16, :3].tolist() == [top, -top, 1.0 / float(s[1])]
+    assert v[16, :3].tolist() == [top * float(s[1]), -top * float(s[1]), 1.0]
 
 
 def test_empty_batch_ends_the_sequences_at_start():
