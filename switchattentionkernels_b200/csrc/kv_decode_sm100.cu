@@ -18,12 +18,12 @@
 // A softmax thread owns one key of a tile (TMEM lane) when it reads S^T, and one of the
 // 128 dims when it reads O^T: O is kept in its registers, one value per head, and each
 // tile's O^T is added with the tile's own factor, so P and the V scales enter as
-// 2^(s - m) vs / ref (never above 1), m the tile's largest score of the head.  The parts' last
-// step is a fixed fraction of ref, and keys under a large scale that get no weight must not
-// take the digits of those that do.  So ref is the tile's largest V scale where its V scales
-// lie within 2^4 of one another (nearly always), else each head's own largest 2^(s - m) vs,
-// which takes a second exchange between the softmax warps (all tiles so: 64 sequences of up to
-// 32K keys 67.8 against 66.7 us, 16 int8 ones with weights 35.9 against 31.7).
+// 2^(s - m) vs / max vs (never above 1), m the tile's largest score of the head.  The parts' last
+// step is a fixed fraction of 1, and keys under a large scale that get no weight must not take
+// the digits of those that do: where a tile's V scales do not lie within 2^4 of one another
+// (hardly ever), m is lowered by head until the largest of these products is 1, which takes a second
+// exchange between the softmax warps (all tiles so: 64 sequences of up to 32K keys 62.2 against
+// 61.0 us, 16 int8 ones with weights 36.2 against 32.2).
 //
 // Measured (B200, graph of ten calls): 64 sequences of 16K-32K keys, an eighth routed full, 359 MB
 // of legal bytes, 61 to 65 us (5.5 to 5.9 TB/s; the e4m3 cache with one scale per head, whose bytes are
@@ -661,10 +661,33 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
           mt[h + 2] = fmaxf(fmaxf(a.z, b.z), fmaxf(c.z, d.z));
           mt[h + 3] = fmaxf(fmaxf(a.w, b.w), fmaxf(c.w, d.w));
         }
-        const bool wide = rb.vref < 0.0f;  // (the same for all threads)
+        // P relative to the tile's maximum, V scales relative to the tile's largest
         const float vref = fabsf(rb.vref);
-        constexpr float kOne = kInt8 ? 1.0f / kInt8One : 1.0f / 256.0f;
         const float vrel = vref > 0.0f ? vs / vref : 0.0f;
+        if (rb.vref < 0.0f) {  // (the same for all threads)
+          // the maximum is lowered by as much as the head's largest 2^(s - m) vs lies below the largest V
+          // scale, to 2^-100 at most, so that all factors stay within FP32
+          const float lv = lg2_approx(vrel);
+          float x[kHeads];
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) {
+            x[h] = s[h] - mt[h] + lv;
+            const float mn = fmaxf(m[h], mt[h]), a = ex2_approx(m[h] - mn);  // (the row's maximum is the true one)
+            m[h] = mn;
+            l[h] *= a;
+            o[h] *= a;
+          }
+          const float mine = reduce_heads<kHeads>(x, lane, larger);
+          if (lane % (32 / kHeads) == 0) off[8 * warp + lane / (32 / kHeads)] = mine;
+          __syncwarp();
+          if (lane == 0) mbar_arrive(off_full);
+          if (!(ok = warp_wait(off_full, nwide & 1, abort_flag))) break;
+          ++nwide;
+          const int lh = lane % kHeads;
+          const float low = fminf(fmaxf(fmaxf(fmaxf(off[lh], off[8 + lh]), fmaxf(off[16 + lh], off[24 + lh])), -100.0f), 0.0f);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) mt[h] += __shfl_sync(0xffffffffu, low, h);
+        }
         float pr[kHeads];
 #pragma unroll
         for (int h = 0; h < kHeads; ++h) {
@@ -674,29 +697,8 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
           m[h] = mn;
           const float e = ex2_approx(s[h] - mt[h]);
           l[h] = fmaf(e, be, l[h] * alpha[h]);
-          beta[h] = be * (vref * kOne);
+          beta[h] = be * (vref * (kInt8 ? 1.0f / kInt8One : 1.0f / 256.0f));
           pr[h] = e * vrel;
-        }
-        if (wide) {  // again, with each head's own ref
-          // ref / 4 in log2, so that its power of two is finite for every FP32 scale; lane h % kHeads: of head h
-          const float lv = lg2_approx(vs) - 2.0f;
-          float x[kHeads];
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) x[h] = s[h] - mt[h] + lv;
-          const float mine = reduce_heads<kHeads>(x, lane, larger);
-          if (lane % (32 / kHeads) == 0) off[8 * warp + lane / (32 / kHeads)] = mine;
-          __syncwarp();
-          if (lane == 0) mbar_arrive(off_full);
-          if (!(ok = warp_wait(off_full, nwide & 1, abort_flag))) break;
-          ++nwide;
-          const int lh = lane % kHeads;
-          const float ref = fmaxf(fmaxf(fmaxf(off[lh], off[8 + lh]), fmaxf(off[16 + lh], off[24 + lh])), -126.0f);
-          const float up = ex2_approx(ref) * (4.0f * kOne), down = ex2_approx(-ref);
-#pragma unroll
-          for (int h = 0; h < kHeads; ++h) {
-            beta[h] = ex2_approx(mt[h] - m[h]) * __shfl_sync(0xffffffffu, up, h);
-            pr[h] = ex2_approx(s[h] - mt[h]) * (vs * 0.25f) * __shfl_sync(0xffffffffu, down, h);
-          }
         }
         uint8_t* pb = smem + Sm::p + buf * kCols * 128;
         auto put = [&](int part, int h, uint32_t byte) {
