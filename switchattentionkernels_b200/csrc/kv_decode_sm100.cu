@@ -10,9 +10,10 @@
 //   S^T [128 keys x N]  = K tile [128 x 128 B] (K-major)  .  Qp^T
 //   O^T [128 dims x N]  = V tile^T (MN-major)             .  Pp^T
 // and the few query heads the N side.  Q and P, which have more than 8 bits, are cut
-// into three 8-bit parts, a column each: e4m3 parts of 4 significant bits (kind::f8f6f4,
-// 12 bits in all: BF16 q exactly, P as FP16) or signed-byte digits (kind::i8, 23 bits and
-// exact INT32 sums).  The parts' results are added up in FP32.
+// into three 8-bit parts, a column each: e4m3 parts of 4 significant bits (kind::f8f6f4, 12 bits in
+// all, P as FP16) or signed-byte digits (kind::i8, 23 bits and exact INT32 sums).  The parts'
+// results are added up in FP32.  Q is scaled by its head's largest |q|: e4m3 parts hold BF16 exactly
+// down to 2^-18 of that and to within 2^-25 of it below, digits all of it to within 2^-23.9.
 //
 // Roles of a CTA (192 threads): warps 0-3 softmax, warp 4 TMA producer, warp 5 MMA issuer.
 // A softmax thread owns one key of a tile (TMEM lane) when it reads S^T, and one of the

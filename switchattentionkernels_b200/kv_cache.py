@@ -216,6 +216,11 @@ def switch_gqa_decode_cached(q: torch.Tensor, cache: SwitchKVCache, route_full: 
     a sequence without rows gets O = NaN, LSE = -inf.  A query with an infinity or NaN
     gets NaN in both.
 
+    The products take the cached bytes as they are.  Attention weights enter the sum over
+    V rounded to 11 bits (e4m3 cache, as FP16) or in steps of 2^-19 or less of the largest
+    contribution (int8), query entries to within 2^-23.9 of their head's largest one;
+    scores, their maxima and sums, LSE and ``key_weights`` are FP32.
+
     With ``accumulate`` and a cache that has ``key_weights``, the softmax weight of every
     row that was attended to, summed over the query heads of its KV head, is added to
     them.  ``status_out``: as in ``switch_gqa_decode_forward``; with a non-zero word

@@ -155,6 +155,35 @@ def test_decode_v_scales_far_apart_in_some_tiles(cuda_device, dtype, B, S, Hq, H
     _within_its_own_size(c, q, torch.rand(B, generator=g) < 0.5, 1000, f"B={B} S={S}")
 
 
+@BOTH
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 8, 2.0 ** 14])
+def test_decode_query_with_a_far_larger_entry(cuda_device, dtype, size):
+    # a large entry that meets no key: the others are held to within 2^-23.9 of it, 2^-25 in e4m3 parts
+    dev = cuda_device
+    g = torch.Generator().manual_seed(41)
+    c = make_switch_kv_cache(2, 900, 2, device=dev, dtype=dtype, block_size=64)
+    k, v = torch.randn(2, 900, 2, 128, generator=g).bfloat16(), torch.randn(2, 900, 2, 128, generator=g).bfloat16()
+    k[..., 0] = 0.0
+    switch_kv_cache_append(c, k.to(dev), v.to(dev))
+    before = ref.clone(c)
+    q = torch.randn(2, 8, 128, generator=g).bfloat16()
+    q[..., 0] = size
+    route = torch.ones(2, dtype=torch.bool)
+    O, L = switch_gqa_decode_cached(q.to(dev), c, route.to(dev))
+    torch.cuda.synchronize()
+    want, lse, _, (eO, eL, _) = ref.decode(before, q, route, 1024)
+    kk = ref.values(before["k"]) * ref.values(before["k_scale"]).repeat_interleave(64, 2)[:, :, :900, None]
+    top = ref.values(q).abs().amax(-1)
+    for b in range(2):
+        for h in range(8):
+            ds = 2.0 ** (-23.9 if dtype == INT8 else -25) * float(top[b, h] * kk[b, h // 4].abs().sum(-1).max()) * ref.LOG2E / math.sqrt(128.0)
+            # a score off by ds moves the LSE by at most that, and every weight by at most twice that in log2
+            assert abs(float(L[b, h]) - float(lse[b, h])) <= float(eL[b, h]) + ds
+            v8 = (ref.values(before["v"][b, h // 4]).abs() * ref.values(before["v_scale"][b, h // 4]).repeat_interleave(64)[:900, None]).amax(0)
+            off = (O[b, h].cpu().double() - want[b, h]).abs()
+            assert bool((off <= eO[b, h] + (2.0 ** (2.0 * ds) - 1.0) * v8 * (1.0 + 2.0 ** -8)).all())
+
+
 def test_decode_that_timed_out_leaves_the_weights(cuda_device):
     # a withheld tile: the call reports it, key_weights are what they were, and the step can be taken again
     from switchattentionkernels_b200 import _native
