@@ -27,7 +27,7 @@
 // 61.0 us, 16 int8 ones with weights 36.2 against 32.2).
 //
 // Measured (B200, graph of ten calls): 64 sequences of 16K-32K keys, an eighth routed full, 359 MB
-// of legal bytes, 61 to 65 us (5.5 to 5.9 TB/s; the e4m3 cache with one scale per head, whose bytes are
+// of legal bytes, 61 to 67 us (5.4 to 5.9 TB/s; the e4m3 cache with one scale per head, whose bytes are
 // converted in registers, takes 154 us); 536 MB of full sequences 85 us (6.3 TB/s).  Reading alone,
 // tiles of this size stream at 7.1 TB/s with 96 to 128 KB in flight per SM and at 6.5 to 7.0 with
 // 192 KB; two CTAs an SM with two K and two V tiles each hold 128 KB (three tiles each: 75.2
