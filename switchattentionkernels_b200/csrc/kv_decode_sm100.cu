@@ -686,8 +686,9 @@ __global__ void __launch_bounds__(kThreads, kKvDecodeCtasPerSm)
           ++nwide;
           const int lh = lane % kHeads;
           const float low = fminf(fmaxf(fmaxf(fmaxf(off[lh], off[8 + lh]), fmaxf(off[16 + lh], off[24 + lh])), -100.0f), 0.0f);
+          // (rounded up: a product above 1 would not fit the signed-byte digits)
 #pragma unroll
-          for (int h = 0; h < kHeads; ++h) mt[h] += __shfl_sync(0xffffffffu, low, h);
+          for (int h = 0; h < kHeads; ++h) mt[h] = __fadd_ru(mt[h], __shfl_sync(0xffffffffu, low, h));
         }
         float pr[kHeads];
 #pragma unroll

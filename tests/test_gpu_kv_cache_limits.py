@@ -156,6 +156,35 @@ def test_decode_v_scales_far_apart_in_some_tiles(cuda_device, dtype, B, S, Hq, H
 
 
 @BOTH
+@pytest.mark.parametrize("Hq", [1, 8])
+def test_decode_v_scales_far_apart_under_scores_of_any_size(cuda_device, dtype, Hq):
+    # scores so large that a unit in their last place is not small, V scales whose ratio is no power of two: the
+    # keys with all the weight share one V row, which is O whatever the scores' rounding is
+    dev = cuda_device
+    g = torch.Generator().manual_seed(Hq)
+    row = torch.randint(-100, 101, (128,), generator=g).float().to(dtype)
+    for size in (1.0, 10.0, 90.0, 100.0, 117.0, 131.0, 150.0, 176.0, 200.0, 255.0, 1000.0):
+        for light, heavy in ((3e-5, 7.0), (0.001, 0.9), (2.0 ** -20, 1.0)):
+            c = make_switch_kv_cache(1, 300, 1, device=dev, dtype=dtype, block_size=16)
+            k = torch.full((300, 128), 100.0)
+            k[16:48], k[130:150] = -100.0, -100.0
+            c.k.copy_(k.to(dtype)[None, None].to(dev))
+            c.v.copy_(row.expand(1, 1, 300, 128).to(dev))
+            c.k_scale.fill_(1.0)
+            c.v_scale.fill_(light)
+            c.v_scale[:, :, 1:3] = heavy
+            c.v[0, 0, 130:150] = 0  # (these under the light scale)
+            c.seq_lens.fill_(300)
+            q = torch.full((1, Hq, 128), size, dtype=torch.bfloat16, device=dev)
+            O, _ = switch_gqa_decode_cached(q, c, torch.ones(1, dtype=torch.bool, device=dev))
+            want = ref.values(row) * float(torch.tensor(light))
+            # equal scores give equal weights, 1 / n each: P's FP16 and last steps, sums, and O to BF16
+            tol = want.abs() * (2.0 ** -8 + 2.0 ** -10) + 1e-12
+            off = (O[0].cpu().double() - want).abs()
+            assert bool((off <= tol).all()), (size, light, heavy, float((off / tol).max()))
+
+
+@BOTH
 @pytest.mark.parametrize("size", [1.0, 2.0 ** 8, 2.0 ** 14])
 def test_decode_query_with_a_far_larger_entry(cuda_device, dtype, size):
     # a large entry that meets no key: the others are held to within 2^-23.9 of it, 2^-25 in e4m3 parts
