@@ -14,6 +14,8 @@
 // all, P as FP16) or signed-byte digits (kind::i8, 23 bits and exact INT32 sums).  The parts'
 // results are added up in FP32.  Q is scaled by its head's largest |q|: e4m3 parts hold BF16 exactly
 // down to 2^-18 of that and to within 2^-25 of it below, digits all of it to within 2^-23.9.
+// P's FP16 rounding is 2^-11 of a weight at most, an eighth of O's to BF16, and differs from key to
+// key: O's error against 64 bits is that of an FP32 step to four digits.
 //
 // Roles of a CTA (192 threads): warps 0-3 softmax, warp 4 TMA producer, warp 5 MMA issuer.
 // A softmax thread owns one key of a tile (TMEM lane) when it reads S^T, and one of the
